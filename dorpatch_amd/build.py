@@ -21,8 +21,10 @@ LIB_PATH = os.path.join(LIB_DIR, "libdorpatch_hip.so")
 # v_pk_fma_f32 costs as much as two v_fma_f32 plus the moves that build its 64-bit operand pairs — in the one
 # VALU-bound kernel here (k_stem_dgrad) that is 233 moves for 168 FMA instructions (explicit float4 arithmetic
 # is vector IR already and unaffected).
+# -packed-fp32-ops: no v_pk_add / mul / fma_f32 from float4 arithmetic either: some of their forms have given wrong results
+# on this hardware now and then.  (The host pass does not know the feature and says so: harmless.)
 HIPCC_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off", "-fno-slp-vectorize",
-               "-fPIC", "-shared", "-Wall"]
+               "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-fPIC", "-shared", "-Wall"]
 
 
 def _hipcc():

@@ -231,40 +231,30 @@ __global__ __launch_bounds__(256) void k_readsum(const f4 *__restrict__ in, floa
   if (acc.x + acc.y + acc.z + acc.w == 12345.678f) out[0] = 1.f;  // keep the loads alive
 }
 
-// fp32 VALU issue rates: N dependent-chain-free FMAs per lane, scalar (v_fma_f32) vs packed (v_pk_fma_f32: 2 FMAs per
-// instruction).  The 157.3 TFLOP/s vector spec counts the packed form; what does this GPU sustain?
-typedef float f2 __attribute__((ext_vector_type(2)));
-template <int PACKED>   // 0: v_fma_f32 all-VGPR, 1: v_pk_fma_f32, 2: v_fmac_f32 with an SGPR multiplier (k_stem_dgrad's form)
+// fp32 VALU issue rates: N dependent-chain-free FMAs per lane.
+template <int FORM>   // 0: v_fma_f32 all-VGPR, 2: v_fmac_f32 with an SGPR multiplier (k_stem_dgrad's form)
 __global__ __launch_bounds__(256) void k_fma_rate(float *__restrict__ out, int iters, float seed) {
   float a[16];
 #pragma unroll
   for (int i = 0; i < 16; ++i) a[i] = seed + (float)(threadIdx.x + i);
   const float m = 1.0000001f, c = 1e-7f;
   for (int it = 0; it < iters; ++it) {
-    if (PACKED == 4) {   // VOP2 fmac, all operands VGPRs
+    if (FORM == 4) {   // VOP2 fmac, all operands VGPRs
 #pragma unroll
       for (int i = 0; i < 16; ++i) asm volatile("v_fmac_f32 %0, %1, %2" : "+v"(a[i]) : "v"(m), "v"(c));
-    } else if (PACKED == 5) {   // VOP3 fma with an SGPR multiplier
+    } else if (FORM == 5) {   // VOP3 fma with an SGPR multiplier
       const float sm = __builtin_amdgcn_readfirstlane(m);
 #pragma unroll
       for (int i = 0; i < 16; ++i) asm volatile("v_fma_f32 %0, %1, %2, %0" : "+v"(a[i]) : "s"(sm), "v"(c));
-    } else if (PACKED == 3) {   // multiplier broadcast from lane 3 of each row of 16 lanes of a VGPR (DPP row_newbcast)
+    } else if (FORM == 3) {   // multiplier broadcast from lane 3 of each row of 16 lanes of a VGPR (DPP row_newbcast)
       float mv = m;
 #pragma unroll
       for (int i = 0; i < 16; ++i)
         asm volatile("v_fmac_f32_dpp %0, %1, %2 row_newbcast:3 row_mask:0xf bank_mask:0xf" : "+v"(a[i]) : "v"(mv), "v"(c));
-    } else if (PACKED == 2) {
+    } else if (FORM == 2) {
       const float sm = __builtin_amdgcn_readfirstlane(m);
 #pragma unroll
       for (int i = 0; i < 16; ++i) asm volatile("v_fmac_f32 %0, %1, %2" : "+v"(a[i]) : "s"(sm), "v"(c));
-    } else if (PACKED == 1) {
-#pragma unroll
-      for (int i = 0; i < 16; i += 2) {
-        f2 v = {a[i], a[i + 1]};
-        asm volatile("v_pk_fma_f32 %0, %0, %1, %2" : "+v"(v) : "v"(f2{m, m}), "v"(f2{c, c}));
-        a[i] = v.x;
-        a[i + 1] = v.y;
-      }
     } else {
 #pragma unroll
       for (int i = 0; i < 16; ++i) asm volatile("v_fma_f32 %0, %0, %1, %2" : "+v"(a[i]) : "v"(m), "v"(c));
@@ -652,16 +642,15 @@ int main(int argc, char **argv) {
   }
   if (g_filter && strstr(g_filter, "fma_rate")) {
     const int it = 4096, blocks = 256 * 16;
-    for (int packed = 0; packed < 6; ++packed) {
+    for (int form : {0, 2, 3, 4, 5}) {
       hipEvent_t e0, e1;
       CK(hipEventCreate(&e0));
       CK(hipEventCreate(&e1));
       auto run = [&] {
-        if (packed == 1) hipLaunchKernelGGL((k_fma_rate<1>), dim3(blocks), dim3(256), 0, st, loss, it, 0.5f);
-        else if (packed == 2) hipLaunchKernelGGL((k_fma_rate<2>), dim3(blocks), dim3(256), 0, st, loss, it, 0.5f);
-        else if (packed == 3) hipLaunchKernelGGL((k_fma_rate<3>), dim3(blocks), dim3(256), 0, st, loss, it, 0.5f);
-        else if (packed == 4) hipLaunchKernelGGL((k_fma_rate<4>), dim3(blocks), dim3(256), 0, st, loss, it, 0.5f);
-        else if (packed == 5) hipLaunchKernelGGL((k_fma_rate<5>), dim3(blocks), dim3(256), 0, st, loss, it, 0.5f);
+        if (form == 2) hipLaunchKernelGGL((k_fma_rate<2>), dim3(blocks), dim3(256), 0, st, loss, it, 0.5f);
+        else if (form == 3) hipLaunchKernelGGL((k_fma_rate<3>), dim3(blocks), dim3(256), 0, st, loss, it, 0.5f);
+        else if (form == 4) hipLaunchKernelGGL((k_fma_rate<4>), dim3(blocks), dim3(256), 0, st, loss, it, 0.5f);
+        else if (form == 5) hipLaunchKernelGGL((k_fma_rate<5>), dim3(blocks), dim3(256), 0, st, loss, it, 0.5f);
         else hipLaunchKernelGGL((k_fma_rate<0>), dim3(blocks), dim3(256), 0, st, loss, it, 0.5f);
       };
       run();
@@ -673,7 +662,7 @@ int main(int argc, char **argv) {
       CK(hipEventElapsedTime(&ms, e0, e1));
       ms /= 5;
       const double flop = 2.0 * 16 * it * 256.0 * blocks;   // v_fmac a += s * c: also 16 FMAs per iteration
-      printf("fma_rate %-22s %8.3f ms  %7.1f TFLOP/s\n", packed == 1 ? "v_pk_fma_f32 (8/iter)" : packed == 2 ? "v_fmac_f32 v,s,v (16/iter)" : packed == 3 ? "v_fmac_f32_dpp row_newbcast" : packed == 4 ? "v_fmac_f32 v,v,v" : packed == 5 ? "v_fma_f32 v,s,v,v" : "v_fma_f32 (16/iter)", ms, flop / (ms * 1e-3) / 1e12);
+      printf("fma_rate %-22s %8.3f ms  %7.1f TFLOP/s\n", form == 2 ? "v_fmac_f32 v,s,v (16/iter)" : form == 3 ? "v_fmac_f32_dpp row_newbcast" : form == 4 ? "v_fmac_f32 v,v,v" : form == 5 ? "v_fma_f32 v,s,v,v" : "v_fma_f32 (16/iter)", ms, flop / (ms * 1e-3) / 1e12);
     }
     return 0;
   }
