@@ -14,12 +14,15 @@ import torch  # noqa: F401
 
 from .build import LIB_PATH
 
-DP_ABI_VERSION = 12
+DP_ABI_VERSION = 13
 DP_MAX_RECTS = 4
 DP_DEBUG_AFFINE_SAMPLES_PER_BLOCK, DP_DEBUG_UPDATE_VARIANT, DP_DEBUG_APPLY_ORDER, DP_DEBUG_AFFINE_GATHER = 1, 2, 3, 4   # dp_debug_set knobs
 DP_DEBUG_CONV1X1_VARIANT = 5
 DP_DEBUG_CONV3X3_VARIANT = 6
 DP_S2BWD_PAIRS, DP_S2BWD_CLASSES = 0, 1      # dp_conv3x3s2_bwd forms
+DP_F32, DP_BF16, DP_F16 = 0, 1, 2            # element types of logits, parameters, gradients
+DP_LOGPROB, DP_PREFERENCE, DP_POLICY = 0, 1, 2   # dp_logits_workspace's operators
+DP_ADAMW_BLOCK = 128                         # elements that share a scale of AdamW's 8-bit states
 
 c_float_p = ctypes.c_void_p  # device pointers travel as integers
 c_int_p = ctypes.c_void_p
@@ -42,8 +45,34 @@ class DpUpdateCfg(ctypes.Structure):
                 ("clip_min", ctypes.c_float), ("clip_max", ctypes.c_float)]
 
 
+class DpLogits(ctypes.Structure):
+    """dp_logits_t"""
+    _fields_ = [("data", ctypes.c_void_p), ("dtype", ctypes.c_int), ("rows", ctypes.c_int), ("vocab", ctypes.c_int),
+                ("inner", ctypes.c_int), ("outer_stride", ctypes.c_int64), ("row_stride", ctypes.c_int64)]
+
+
+class DpPolicyCfg(ctypes.Structure):
+    """dp_policy_cfg_t"""
+    _fields_ = [(name, ctypes.c_float) for name in ("clip_low", "clip_high", "kl_coef", "entropy_coef", "upstream")]
+
+
+class DpAdamwTensor(ctypes.Structure):
+    """dp_adamw_tensor_t"""
+    _fields_ = [("param", ctypes.c_void_p), ("grad", ctypes.c_void_p), ("n", ctypes.c_int64), ("at", ctypes.c_int64),
+                ("lr", ctypes.c_double), ("weight_decay", ctypes.c_double), ("param_dtype", ctypes.c_int),
+                ("grad_dtype", ctypes.c_int)]
+
+
+class DpAdamwCfg(ctypes.Structure):
+    """dp_adamw_cfg_t"""
+    _fields_ = [("beta1", ctypes.c_double), ("beta2", ctypes.c_double), ("eps", ctypes.c_double), ("max_norm", ctypes.c_double),
+                ("box_low", ctypes.c_float), ("box_high", ctypes.c_float), ("box", ctypes.c_int), ("state_bits", ctypes.c_int),
+                ("step", ctypes.c_int64), ("seed", ctypes.c_uint32)]
+
+
 # name -> (restype, argtypes); mirrors include/dorpatch_hip.h one to one
 _I, _F, _P, _L = ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_int64
+_LOGITS, _ADAMW = ctypes.POINTER(DpLogits), ctypes.POINTER(DpAdamwCfg)
 PROTOTYPES = {
     "dp_abi_version": (_I, []),
     "dp_error_string": (ctypes.c_char_p, [_I]),
@@ -82,6 +111,13 @@ PROTOTYPES = {
     "dp_stem_dgrad_reduce": (_I, [_P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, ctypes.POINTER(DpNorm), _P, _P]),
     "dp_subsample2": (_I, [_P, _L, _I, _I, _P, _P]),
     "dp_subsample2_add": (_I, [_P, _L, _I, _I, _P, _P]),
+    "dp_logits_workspace": (_L, [_I, _I, _I, _I]),
+    "dp_label_logprob": (_I, [_LOGITS, _P, _P, _P, _P, _P, _P]),
+    "dp_label_logprob_bwd": (_I, [_LOGITS, _P, _P, _P, _LOGITS, _P]),
+    "dp_preference_loss": (_I, [_LOGITS, _P, _P, _I, _P, _F, _F, _F, _I, _P, _P, _LOGITS, _P, _P]),
+    "dp_policy_loss": (_I, [ctypes.POINTER(DpPolicyCfg), _LOGITS] + [_P] * 8 + [_LOGITS, _P, _P]),
+    "dp_adamw_workspace": (_L, [_ADAMW, ctypes.POINTER(DpAdamwTensor), _I]),
+    "dp_adamw_step": (_I, [_ADAMW, ctypes.POINTER(DpAdamwTensor), _I] + [_P] * 8),
     "dp_event_create": (_I, [ctypes.POINTER(ctypes.c_void_p)]),
     "dp_event_destroy": (_I, [_P]),
     "dp_event_elapsed_ms": (_I, [_P, _P, ctypes.POINTER(ctypes.c_float)]),

@@ -43,14 +43,14 @@ def needs_build():
     return any(os.path.getmtime(d) > t for d in deps)
 
 
-PARTS = (1, 2, 3, 4, 5)  # -DDP_PART values: the kernel families of csrc/*.inc as five translation units (csrc/dorpatch_hip.hip, top), compiled in parallel
+PARTS = (1, 2, 3, 4, 5, 6)  # -DDP_PART values: the kernel families of csrc/*.inc as six translation units (csrc/dorpatch_hip.hip, top), compiled in parallel
 
 
 def build_extension(force=False, verbose=False, jobs=None):
     """Compile the HIP kernels + C ABI. Returns the path of the shared library.
 
-    Round 6: one file per kernel family (``csrc/*.inc``), compiled as five translation units
-    (``-DDP_PART=1..5``) by concurrent hipcc processes and linked into the one library — 26 s of wall time instead of 75 on
+    Round 6: one file per kernel family (``csrc/*.inc``), compiled as six translation units
+    (``-DDP_PART=1..6``) by concurrent hipcc processes and linked into the one library — 26 s of wall time instead of 75 on
     the 8-core build container."""
     if not force and not needs_build():
         return LIB_PATH

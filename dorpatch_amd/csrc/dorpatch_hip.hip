@@ -23,11 +23,11 @@
 
 #include "dorpatch_hip.h"
 
-// One library, one file per kernel family, five translation units (round 6).  This file holds what the
+// One library, one file per kernel family, six translation units.  This file holds what the
 // families share (macros, reductions, the debug knobs) and the list of family files below; the product build
-// (dorpatch_amd/build.py) compiles it five times IN PARALLEL with -DDP_PART=1..5 — 1: apply.inc + update.inc (the DorPatch
+// (dorpatch_amd/build.py) compiles it six times IN PARALLEL with -DDP_PART=1..6 — 1: apply.inc + update.inc (the DorPatch
 // arithmetic), gn.inc, stem.inc; 2: conv3x3.inc (direct 3x3, stride 1); 3: conv1x1.inc; 4: conv3x3_wino.inc; 5: conv3x3s2.inc
-// (stride-2 3x3 and its input gradient) — and links the objects into the one libdorpatch_hip.so; a kernel, its launcher and
+// (stride-2 3x3 and its input gradient); 6: logits.inc + adamw.inc (losses and optimiser of a training step) — and links the objects into the one libdorpatch_hip.so; a kernel, its launcher and
 // its extern "C" entry point live in the same file.  DP_PART = 0 (the default: tools/kbench's white-box include, the host
 // emulation of tests/hipemu) is the whole library in one unit.
 #ifndef DP_PART
@@ -134,6 +134,10 @@ __device__ __forceinline__ float sgn(float v) {
 #endif
 #if DP_HAS(4)
 #include "conv3x3_wino.inc"   // Winograd F(2x2, 3x3) on the matrix cores
+#endif
+#if DP_HAS(6)
+#include "logits.inc"         // log-probabilities, preference loss, clipped policy loss on rows of logits
+#include "adamw.inc"          // AdamW over many tensors
 #endif
 
 // ============================================================================

@@ -268,6 +268,189 @@ def cw_loss(logits, y, targeted, S, confidence, upstream, loss_out=None, want_gr
     return loss, dlogits, pred
 
 
+# ---------------------------------------------------------------- losses on rows of logits (a training step; not in the reference)
+ELEMENT_TYPES = {torch.float32: _lib.DP_F32, torch.bfloat16: _lib.DP_BF16, torch.float16: _lib.DP_F16}
+
+
+def _here(t, name):
+    """The launch goes to the current device's stream: a tensor of another device is refused."""
+    if t.is_cuda and t.device.index != torch.cuda.current_device():
+        raise RuntimeError("`%s` is on %s, the current device is cuda:%d (torch.cuda.device selects it)"
+                           % (name, t.device, torch.cuda.current_device()))
+
+
+def _logits(x, name="logits"):
+    """(dp_logits_t, rows) of a (..., V) tensor of 1 to 3 dimensions, its last one dense; the others may have any strides."""
+    if not isinstance(x, torch.Tensor) or x.dtype not in ELEMENT_TYPES:
+        raise TypeError("`%s` must be a float32, bfloat16 or float16 tensor" % name)
+    _chk(x.as_strided((0,), (1,)), x.dtype, name)            # a GPU tensor, dense or not
+    if not 1 <= x.dim() <= 3:
+        raise ValueError("`%s` must have 1 to 3 dimensions (..., V), got %s" % (name, tuple(x.shape)))
+    V = x.shape[-1]
+    if V < 1 or (V > 1 and x.stride(-1) != 1):
+        raise ValueError("`%s` needs at least one category and a dense last dimension" % name)
+    rows = x.numel() // V
+    inner = x.shape[-2] if x.dim() > 1 else 1
+    outer_stride = x.stride(0) if x.dim() == 3 else 0
+    row_stride = x.stride(-2) if x.dim() > 1 else 0
+    return _lib.DpLogits(x.data_ptr(), ELEMENT_TYPES[x.dtype], rows, V, max(inner, 1), outer_stride, row_stride), rows
+
+
+def _labels(labels, logits):
+    _chk(labels, torch.int64, "labels")
+    if tuple(labels.shape) != tuple(logits.shape[:-1]):
+        raise ValueError("`labels` must have the shape of the logits' rows %s, got %s"
+                         % (tuple(logits.shape[:-1]), tuple(labels.shape)))
+    _here(labels, "labels"), _here(logits, "logits")
+
+
+def _per_row(t, shape, name):
+    if t is None:
+        return
+    _chk(t, torch.float32, name)
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError("`%s` must have the shape %s, got %s" % (name, tuple(shape), tuple(t.shape)))
+    _here(t, name)
+
+
+def _dlogits(logits, out):
+    """The gradient's tensor: a new dense one, or the caller's ``out`` (the logits themselves, or memory apart from them)."""
+    if out is None:
+        return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    if not isinstance(out, torch.Tensor) or out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
+        raise ValueError("`out` must be a tensor like the logits (%s, %s)" % (tuple(logits.shape), logits.dtype))
+    reach = out.shape[-1]                                    # elements that the dimensions so far span: the next stride must clear them
+    for stride, size in sorted(zip(out.stride()[:-1], out.shape[:-1])):
+        if size > 1:
+            if stride < reach:
+                raise ValueError("`out` must not overlap itself")
+            reach += (size - 1) * stride
+    same = out.data_ptr() == logits.data_ptr() and out.stride() == logits.stride()
+    if not same and out.numel():
+        a, b = out.data_ptr(), logits.data_ptr()
+        if a < b + _extent(logits) and b < a + _extent(out):
+            raise ValueError("`out` must be the logits themselves or memory apart from them")
+    return out
+
+
+def _extent(t):
+    return (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size() if t.numel() else 0
+
+
+def _logits_workspace(op, d, device):
+    n = _lib.load().dp_logits_workspace(op, d.rows, d.vocab, d.dtype)
+    return torch.empty((n,), dtype=torch.uint8, device=device) if n else None
+
+
+def label_logprob(logits, labels, want_entropy=False):
+    """Log-probabilities of the labels under softmax(logits): (logp, entropy or None, stats).
+
+    ``logits`` (R, V), (B, T, V) or (V,) in float32 / bfloat16 / float16, the last dimension dense, the others with any strides
+    (``x[:, :-1]`` of a (B, T, V) tensor is taken as it lies); ``labels`` int64 of the rows' shape, a negative one marks a row
+    that counts for nothing: it is not read, its outputs are 0 and so is its gradient.  A row that allows nothing (all -inf)
+    counts the same; a label beyond the vocabulary gives NaN.  ``logp`` and ``entropy``: float32 of the rows' shape; ``stats``
+    (R, 2): what ``label_logprob_bwd`` needs."""
+    lib = _lib.load()
+    d, rows = _logits(logits)
+    _labels(labels, logits)
+    logp = torch.empty(labels.shape, dtype=torch.float32, device=logits.device)
+    entropy = torch.empty_like(logp) if want_entropy else None
+    stats = torch.empty((rows, 2), dtype=torch.float32, device=logits.device)
+    if rows:
+        work = _logits_workspace(_lib.DP_LOGPROB, d, logits.device)
+        _lib.check(lib.dp_label_logprob(ctypes.byref(d), _p(labels), _p(logp), _p(entropy), _p(stats), _p(work), _stream()),
+                   "dp_label_logprob")
+    return logp, entropy, stats
+
+
+def label_logprob_bwd(logits, labels, stats, g, out=None):
+    """d sum(g * logp) / d logits for ``stats`` from ``label_logprob`` on the same logits; ``g`` float32 of the rows' shape.
+    ``out`` may be the logits themselves."""
+    lib = _lib.load()
+    d, rows = _logits(logits)
+    _labels(labels, logits)
+    _per_row(stats, (rows, 2), "stats"), _per_row(g, labels.shape, "g")
+    out = _dlogits(logits, out)
+    if rows:
+        _lib.check(lib.dp_label_logprob_bwd(ctypes.byref(d), _p(labels), _p(stats), _p(g), ctypes.byref(_logits(out, "out")[0]),
+                                            _stream()), "dp_label_logprob_bwd")
+    return out
+
+
+def preference_loss(logits, labels, cu_seqlens, ref_logp, beta, upstream, label_smoothing=0.0, average=False, want_grad=True,
+                    out=None):
+    """Preference loss over pairs of sequences (paired log ratios) and its gradient: (loss (P,), dlogits or None, seq_logp (2P,)).
+
+    ``logits`` (R, V), ``labels`` (R,) as in ``label_logprob``; ``cu_seqlens`` (2P + 1,) int32: the sequences' first rows,
+    ascending, the preferred and the other one of a pair side by side (an empty one is fine; rows outside all of them get a
+    zero gradient).  With L the sum of a sequence's log-probabilities (``average``: their mean over the labels that count) and
+    h = beta * ((L0 - ref0) - (L1 - ref1)), ``ref_logp`` (2P,) or None for zeroes:
+    loss = -(1 - label_smoothing) log sigmoid(h) - label_smoothing log sigmoid(-h);
+    dlogits = upstream * d sum(loss) / d logits (``out`` may be the logits themselves)."""
+    lib = _lib.load()
+    d, rows = _logits(logits)
+    if logits.dim() != 2:
+        raise ValueError("`logits` must be (R, V): the sequences lie one after the other")
+    _labels(labels, logits)
+    _chk(cu_seqlens, torch.int32, "cu_seqlens"), _here(cu_seqlens, "cu_seqlens")
+    if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1 or cu_seqlens.shape[0] % 2 != 1:
+        raise ValueError("`cu_seqlens` must be (2 * pairs + 1,), got %s" % (tuple(cu_seqlens.shape),))
+    P = cu_seqlens.shape[0] // 2
+    _per_row(ref_logp, (2 * P,), "ref_logp")
+    if not 0.0 <= label_smoothing <= 1.0:
+        raise ValueError("`label_smoothing` must be in [0, 1], got %r" % (label_smoothing,))
+    loss = torch.empty((P,), dtype=torch.float32, device=logits.device)
+    seq_logp = torch.empty((2 * P,), dtype=torch.float32, device=logits.device)
+    dlogits = _dlogits(logits, out) if want_grad else None
+    if rows == 0 or P == 0:          # nothing that a kernel would read: sums of nothing
+        seq_logp.zero_()
+        if P:
+            h = float(beta) * (0.0 if ref_logp is None else ref_logp[1::2] - ref_logp[0::2]) + torch.zeros_like(loss)
+            loss.copy_(torch.nn.functional.softplus(-h) + float(label_smoothing) * h)
+        return loss, (dlogits.zero_() if want_grad else None), seq_logp
+    work = _logits_workspace(_lib.DP_PREFERENCE, d, logits.device)
+    dd = ctypes.byref(_logits(dlogits, "out")[0]) if want_grad else None
+    _lib.check(lib.dp_preference_loss(ctypes.byref(d), _p(labels), _p(cu_seqlens), P, _p(ref_logp), float(beta), float(upstream),
+                                      float(label_smoothing), 1 if average else 0, _p(loss), _p(seq_logp), dd, _p(work),
+                                      _stream()), "dp_preference_loss")
+    return loss, dlogits, seq_logp
+
+
+def policy_loss(logits, labels, old_logp, advantage, clip_low, clip_high, upstream, ref_logp=None, kl_coef=0.0, entropy_coef=0.0,
+                weight=None, want_entropy=None, want_grad=True, out=None):
+    """Clipped policy loss with a KL term and an entropy bonus, and its gradient:
+    (loss, dlogits or None, logp, entropy or None), all but dlogits float32 of the rows' shape.
+
+    ``logits`` and ``labels`` (what was drawn) as in ``label_logprob``; with ratio = exp(logp - old_logp):
+    loss = max(-advantage * ratio, -advantage * clamp(ratio, 1 - clip_low, 1 + clip_high))
+           + kl_coef * (exp(ref_logp - logp) - (ref_logp - logp) - 1) - entropy_coef * entropy;
+    dlogits = upstream * d sum(weight * loss) / d logits.  ``old_logp``, ``advantage``, ``ref_logp``, ``weight``: float32 of the
+    rows' shape.  ``want_entropy`` None: if entropy_coef is not 0.  ``out`` may be the logits themselves."""
+    lib = _lib.load()
+    d, rows = _logits(logits)
+    _labels(labels, logits)
+    for name, t in (("old_logp", old_logp), ("advantage", advantage), ("ref_logp", ref_logp), ("weight", weight)):
+        if t is None and name in ("old_logp", "advantage"):
+            raise TypeError("`%s` is needed" % name)
+        _per_row(t, labels.shape, name)
+    if not (0.0 <= clip_low <= 1.0 and clip_high >= 0.0):
+        raise ValueError("need 0 <= clip_low <= 1 and clip_high >= 0, got %r, %r" % (clip_low, clip_high))
+    if kl_coef != 0.0 and ref_logp is None:
+        raise ValueError("`kl_coef` needs `ref_logp`")
+    want_entropy = entropy_coef != 0.0 if want_entropy is None else want_entropy
+    loss = torch.empty(labels.shape, dtype=torch.float32, device=logits.device)
+    logp = torch.empty_like(loss)
+    entropy = torch.empty_like(loss) if want_entropy else None
+    dlogits = _dlogits(logits, out) if want_grad else None
+    if rows:
+        cfg = _lib.DpPolicyCfg(float(clip_low), float(clip_high), float(kl_coef), float(entropy_coef), float(upstream))
+        work = _logits_workspace(_lib.DP_POLICY, d, logits.device)
+        dd = ctypes.byref(_logits(dlogits, "out")[0]) if want_grad else None
+        _lib.check(lib.dp_policy_loss(ctypes.byref(cfg), ctypes.byref(d), _p(labels), _p(old_logp), _p(advantage), _p(ref_logp),
+                                      _p(weight), _p(loss), _p(logp), _p(entropy), dd, _p(work), _stream()), "dp_policy_loss")
+    return loss, dlogits, logp, entropy
+
+
 def argmax(logits):
     lib = _lib.load()
     _chk(logits, torch.float32, "logits")

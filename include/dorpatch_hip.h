@@ -27,7 +27,7 @@
 extern "C" {
 #endif
 
-#define DP_ABI_VERSION 12
+#define DP_ABI_VERSION 13
 #define DP_MAX_RECTS 4 /* occlusion windows per mask-table entry */
 
 typedef void *dp_stream_t; /* hipStream_t */
@@ -403,6 +403,100 @@ int dp_stem_dgrad_reduce(const float *dy, const float *w, const int32_t *table, 
  * dp_subsample2_add also writes them back. */
 int dp_subsample2(const float *x, int64_t NC, int H, int W, float *y, dp_stream_t stream);
 int dp_subsample2_add(const float *dy, int64_t NC, int H, int W, float *g, dp_stream_t stream);
+
+/* ---- a training step of a categorical model: log-probabilities, preference and policy losses with gradients, AdamW ----
+ * (beside dp_cw_loss and dp_project_update; not in the reference, whose losses and update are those two.)  The categories are
+ * whatever the logits are over: classes, the cells a patch may take, the double masks, tokens.
+ *
+ * Rows of logits: row r of `rows` lies at  data + (r / inner) * outer_stride + (r % inner) * row_stride  elements (strides >= 0;
+ * a dense (R, V) tensor: inner = R, row_stride = V; the slice x[:, :-1] of a (B, T, V) tensor: inner = T - 1, row_stride = V,
+ * outer_stride = T * V), its `vocab` elements side by side; any element alignment.  rows <= 2^23, vocab <= 2^30.
+ * labels (rows) int64.  A label < 0 marks a row that counts for nothing (a prompt, padding): its logits are not read, its
+ * outputs and its gradient are 0 whatever is in it.  So does a row whose logits are all -inf.  A label >= vocab gives NaN in
+ * the row's outputs and gradient, and no access.  Single logits may be -inf (not allowed: probability 0).
+ * Gradients go to a tensor `d` of the same type and size, with strides of its own; it may be the logits themselves.
+ * Sums are fp32, scalars of a row fp64; no atomics: the same inputs give the same bits.
+ * workspace: dp_logits_workspace(op, rows, vocab, dtype) bytes, 16-byte aligned (NULL where that is 0). */
+#define DP_F32 0
+#define DP_BF16 1
+#define DP_F16 2
+#define DP_LOGPROB 0
+#define DP_PREFERENCE 1
+#define DP_POLICY 2
+typedef struct {
+  void *data;
+  int dtype; /* DP_F32, DP_BF16, DP_F16 */
+  int rows, vocab, inner;
+  int64_t outer_stride, row_stride; /* elements */
+} dp_logits_t;
+
+int64_t dp_logits_workspace(int op, int rows, int vocab, int dtype);
+
+/* logp[r] = log softmax(x_r)[label], entropy[r] = entropy of softmax(x_r) (may be NULL), stats (rows, 2) = the row's maximum m
+ * and sum of exp(x - m) (may be NULL; 0 for a row that counts for nothing): what the backward needs.  Reads the logits once. */
+int dp_label_logprob(const dp_logits_t *x, const int64_t *labels, float *logp, float *entropy, float *stats, void *workspace,
+                     dp_stream_t stream);
+/* d[r][j] = g[r] * ([j == label] - softmax(x_r)[j]).  Reads and writes once; rows with g = 0 are not read. */
+int dp_label_logprob_bwd(const dp_logits_t *x, const int64_t *labels, const float *stats, const float *g, const dp_logits_t *d,
+                         dp_stream_t stream);
+
+/* Preference loss of pairs of sequences.  Sequence k is the rows [cu_seqlens[k], cu_seqlens[k + 1]) (int32, 2 * pairs + 1
+ * ascending values; empty ones and rows outside are fine), 2 i the preferred and 2 i + 1 the other of pair i.
+ *   L_k = sum over its rows that count of log softmax(x)[label]  (average: their mean; 0 for none)       -> seq_logp (2 pairs)
+ *   h_i = beta * ((L_2i - ref_logp[2i]) - (L_2i+1 - ref_logp[2i+1]))          (ref_logp NULL: 0)
+ *   loss[i] = -(1 - label_smoothing) log sigmoid(h_i) - label_smoothing log sigmoid(-h_i)
+ * d (may be NULL: forward only) = upstream * d sum(loss) / d x: every row of it is written.
+ * Reads the logits twice and writes the gradient once: a row's gradient needs the sums of its whole pair. */
+int dp_preference_loss(const dp_logits_t *x, const int64_t *labels, const int32_t *cu_seqlens, int pairs, const float *ref_logp,
+                       float beta, float upstream, float label_smoothing, int average, float *loss, float *seq_logp,
+                       const dp_logits_t *d, void *workspace, dp_stream_t stream);
+
+/* Clipped policy loss.  With lp = log softmax(x_r)[label], ratio = exp(lp - old_logp[r]), A = advantage[r]:
+ *   loss[r] = max(-A ratio, -A min(max(ratio, 1 - clip_low), 1 + clip_high))
+ *             + kl_coef (exp(ref_logp[r] - lp) - (ref_logp[r] - lp) - 1) - entropy_coef entropy_r       (ref_logp NULL: no KL term)
+ * d (may be NULL) = upstream * d sum(weight * loss) / d x   (weight (rows) may be NULL: 1; it scales the gradient alone, as
+ * upstream does); where the clipped branch is the larger one its gradient is 0, where both are equal that of the first is taken.
+ * logp, entropy (may be NULL) as in dp_label_logprob. */
+typedef struct {
+  float clip_low, clip_high, kl_coef, entropy_coef, upstream;
+} dp_policy_cfg_t;
+int dp_policy_loss(const dp_policy_cfg_t *cfg, const dp_logits_t *x, const int64_t *labels, const float *old_logp,
+                   const float *advantage, const float *ref_logp, const float *weight, float *loss, float *logp, float *entropy,
+                   const dp_logits_t *d, void *workspace, dp_stream_t stream);
+
+/* AdamW over many tensors at once.  The table of tensors is HOST memory (copied into the launches: nothing of it is kept):
+ * n elements of param and grad (dense; any element alignment; DP_F32 / DP_BF16 / DP_F16 each; n <= 2^34), the place
+ * `at` of its part in the states (a multiple of DP_ADAMW_BLOCK, parts padded to a multiple of it and disjoint), lr and weight_decay.  Per element, every operation rounded to fp32:
+ *   g' = g * clip,  m = beta1 m + (1 - beta1) g',  v = beta2 v + (1 - beta2) g'^2,
+ *   param = param (1 - lr weight_decay) - (m / (sqrt(v) / sqrt(1 - beta2^t) + eps)) * (lr / (1 - beta1^t)),  then clamped to
+ *   [box_low, box_high] if box; rounded to nearest where param is narrower than fp32.
+ * state_bits 32: m, v are fp32.  8: m, v are OCP e4m3 bytes and m_scale, v_scale one float for each DP_ADAMW_BLOCK elements, the power of
+ *   two that brings the block's largest finite magnitude into [128, 256).  Rounding is stochastic (expectation-preserving: with beta2
+ *   near 1 the nearest code would never move): up with the probability of the part cut off, from 16 bits of a hash of
+ *   (seed, t, at + element) each for m and v.  A v > 0 never becomes 0 (the smallest code instead: a smaller step, not a larger
+ *   one); a value that is not finite is stored as NaN.
+ * t: step if counter is NULL; else the int64 on the device is advanced by one first and taken (captured graphs: it advances on
+ *   every replay).  max_norm > 0 needs it: clip = min(1, max_norm / (norm + 1e-6)) with norm = sqrt(sum of all g^2), summed in
+ *   fp64 in a fixed order -> *norm.  Where norm is not finite nothing is changed, t neither.
+ * workspace: dp_adamw_workspace() bytes, 16-byte aligned.  Refused (hipErrorInvalidValue): params that overlap, states that do. */
+#define DP_ADAMW_BLOCK 128
+typedef struct {
+  void *param;
+  const void *grad;
+  int64_t n, at;
+  double lr, weight_decay;
+  int param_dtype, grad_dtype;
+} dp_adamw_tensor_t;
+typedef struct {
+  double beta1, beta2, eps, max_norm; /* max_norm <= 0: no clipping */
+  float box_low, box_high;
+  int box, state_bits;
+  int64_t step;
+  uint32_t seed;
+} dp_adamw_cfg_t;
+int64_t dp_adamw_workspace(const dp_adamw_cfg_t *cfg, const dp_adamw_tensor_t *tensors, int count);
+int dp_adamw_step(const dp_adamw_cfg_t *cfg, const dp_adamw_tensor_t *tensors, int count, void *m, float *m_scale, void *v,
+                  float *v_scale, int64_t *counter, float *norm, void *workspace, dp_stream_t stream);
 
 /* ---- measurement support (bench.py "roofline"): kernel-precise duration of dp_apply_fwd ----
  * dp_apply_fwd_timed is dp_apply_fwd launched through hipExtLaunchKernelGGL, which stamps `start` /
