@@ -432,8 +432,8 @@ typedef struct {
 
 int64_t dp_logits_workspace(int op, int rows, int vocab, int dtype);
 
-/* logp[r] = log softmax(x_r)[label], entropy[r] = entropy of softmax(x_r) (may be NULL), stats (rows, 2) = the row's maximum m
- * and sum of exp(x - m) (may be NULL; 0 for a row that counts for nothing): what the backward needs.  Reads the logits once. */
+/* logp[r] = log softmax(x_r)[label], entropy[r] = entropy of softmax(x_r) (may be NULL), stats (rows, 2): what the backward needs
+ * of the row (may be NULL).  Reads the logits once. */
 int dp_label_logprob(const dp_logits_t *x, const int64_t *labels, float *logp, float *entropy, float *stats, void *workspace,
                      dp_stream_t stream);
 /* d[r][j] = g[r] * ([j == label] - softmax(x_r)[j]).  Reads and writes once; rows with g = 0 are not read. */

@@ -144,7 +144,8 @@ def test_banned_entries_and_strange_rows(V, dtype):
     d = ops.label_logprob_bwd(xd, yd, stats, torch.ones(9).to(DEV)).cpu().double()
     p, want, entropy, dead = softmax64(x, y)
     logp, ent = logp.cpu(), ent.cpu()
-    assert logp[0] == 0 and abs(ent[0]) <= LOG_S and (d[0] == 0).all()
+    # the one term of s is within 2 u of a power of two's: log s as near to 0, and 1 - e (1 / s) is off by 3 roundings
+    assert -LOG_S <= logp[0] <= 0 and 0 <= ent[0] <= LOG_S and (d[0].abs() <= 4 * U).all()
     assert logp[1] == 0 and ent[1] == 0 and (d[1] == 0).all()
     check_logp(logp[2:4], want[2:4]), check_logp(ent[2:4], entropy[2:4])
     assert (logp[4:6] == 0).all() and (ent[4:6] == 0).all() and (d[4:6] == 0).all()
