@@ -274,49 +274,71 @@ ELEMENT_TYPES = {torch.float32: _lib.DP_F32, torch.bfloat16: _lib.DP_BF16, torch
 
 def _here(t, name):
     """The launch goes to the current device's stream: a tensor of another device is refused."""
-    if t.is_cuda and t.device.index != torch.cuda.current_device():
+    if t.is_cuda and t.get_device() != _device():
         raise RuntimeError("`%s` is on %s, the current device is cuda:%d (torch.cuda.device selects it)"
                            % (name, t.device, torch.cuda.current_device()))
 
 
-def _logits(x, name="logits"):
+def _device():
+    return _cur_device() if _cur_device is not None else torch.cuda.current_device()
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _rows(x, name="logits"):
     """(dp_logits_t, rows) of a (..., V) tensor of 1 to 3 dimensions, its last one dense; the others may have any strides."""
-    if not isinstance(x, torch.Tensor) or x.dtype not in ELEMENT_TYPES:
+    kind = ELEMENT_TYPES.get(x.dtype) if isinstance(x, torch.Tensor) else None
+    if kind is None:
         raise TypeError("`%s` must be a float32, bfloat16 or float16 tensor" % name)
-    _chk(x.as_strided((0,), (1,)), x.dtype, name)            # a GPU tensor, dense or not
-    if not 1 <= x.dim() <= 3:
-        raise ValueError("`%s` must have 1 to 3 dimensions (..., V), got %s" % (name, tuple(x.shape)))
-    V = x.shape[-1]
-    if V < 1 or (V > 1 and x.stride(-1) != 1):
+    shape, stride = x.shape, x.stride()
+    n = len(shape)
+    if not 1 <= n <= 3:
+        raise ValueError("`%s` must have 1 to 3 dimensions (..., V), got %s" % (name, tuple(shape)))
+    V = shape[-1]
+    if V < 1 or (V > 1 and stride[-1] != 1):
         raise ValueError("`%s` needs at least one category and a dense last dimension" % name)
-    rows = x.numel() // V
-    inner = x.shape[-2] if x.dim() > 1 else 1
-    outer_stride = x.stride(0) if x.dim() == 3 else 0
-    row_stride = x.stride(-2) if x.dim() > 1 else 0
-    return _lib.DpLogits(x.data_ptr(), ELEMENT_TYPES[x.dtype], rows, V, max(inner, 1), outer_stride, row_stride), rows
+    if n == 2:
+        rows, inner, outer, row = shape[0], shape[0], 0, stride[0]
+    elif n == 3:
+        rows, inner, outer, row = shape[0] * shape[1], shape[1], stride[0], stride[1]
+    else:
+        rows, inner, outer, row = 1, 1, 0, 0
+    return _lib.DpLogits(x.data_ptr(), kind, rows, V, inner or 1, outer, row), rows
 
 
-def _labels(labels, logits):
+def _logits(logits, labels):
+    """Checks the pair; (dp_logits_t, rows, the rows' shape)."""
+    d, rows = _rows(logits)
     _chk(labels, torch.int64, "labels")
-    if tuple(labels.shape) != tuple(logits.shape[:-1]):
+    shape = labels.shape
+    if shape != logits.shape[:-1]:
         raise ValueError("`labels` must have the shape of the logits' rows %s, got %s"
-                         % (tuple(logits.shape[:-1]), tuple(labels.shape)))
-    _here(labels, "labels"), _here(logits, "logits")
+                         % (tuple(logits.shape[:-1]), tuple(shape)))
+    _beside(logits, labels, "logits"), _here(labels, "labels")
+    return d, rows, shape
 
 
-def _per_row(t, shape, name):
+def _beside(t, labels, name):
+    if t.device != labels.device:
+        raise RuntimeError("`%s` is on %s, `labels` on %s" % (name, t.device, labels.device))
+
+
+def _per_row(t, shape, labels, name):
     if t is None:
         return
     _chk(t, torch.float32, name)
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError("`%s` must have the shape %s, got %s" % (name, tuple(shape), tuple(t.shape)))
-    _here(t, name)
+    _beside(t, labels, name)
 
 
-def _dlogits(logits, out):
-    """The gradient's tensor: a new dense one, or the caller's ``out`` (the logits themselves, or memory apart from them)."""
+def _dlogits(logits, d, out):
+    """(tensor, dp_logits_t) of the gradient: a new dense one, or the caller's ``out`` (the logits themselves, or memory apart)."""
     if out is None:
-        return torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        out = torch.empty_like(logits, memory_format=torch.contiguous_format)
+        return out, _lib.DpLogits(out.data_ptr(), d.dtype, d.rows, d.vocab, d.rows or 1, 0, d.vocab)
     if not isinstance(out, torch.Tensor) or out.shape != logits.shape or out.dtype != logits.dtype or out.device != logits.device:
         raise ValueError("`out` must be a tensor like the logits (%s, %s)" % (tuple(logits.shape), logits.dtype))
     reach = out.shape[-1]                                    # elements that the dimensions so far span: the next stride must clear them
@@ -330,7 +352,7 @@ def _dlogits(logits, out):
         a, b = out.data_ptr(), logits.data_ptr()
         if a < b + _extent(logits) and b < a + _extent(out):
             raise ValueError("`out` must be the logits themselves or memory apart from them")
-    return out
+    return out, _rows(out, "out")[0]
 
 
 def _extent(t):
@@ -351,14 +373,14 @@ def label_logprob(logits, labels, want_entropy=False):
     counts the same; a label beyond the vocabulary gives NaN.  ``logp`` and ``entropy``: float32 of the rows' shape; ``stats``
     (R, 2): what ``label_logprob_bwd`` needs."""
     lib = _lib.load()
-    d, rows = _logits(logits)
-    _labels(labels, logits)
-    logp = torch.empty(labels.shape, dtype=torch.float32, device=logits.device)
-    entropy = torch.empty_like(logp) if want_entropy else None
+    d, rows, shape = _logits(logits, labels)
     stats = torch.empty((rows, 2), dtype=torch.float32, device=logits.device)
+    logp = stats.new_empty(shape)
+    entropy = torch.empty_like(logp) if want_entropy else None
     if rows:
         work = _logits_workspace(_lib.DP_LOGPROB, d, logits.device)
-        _lib.check(lib.dp_label_logprob(ctypes.byref(d), _p(labels), _p(logp), _p(entropy), _p(stats), _p(work), _stream()),
+        _lib.check(lib.dp_label_logprob(ctypes.byref(d), labels.data_ptr(), logp.data_ptr(), _ptr(entropy), stats.data_ptr(), _ptr(work),
+                                        _stream()),
                    "dp_label_logprob")
     return logp, entropy, stats
 
@@ -367,12 +389,11 @@ def label_logprob_bwd(logits, labels, stats, g, out=None):
     """d sum(g * logp) / d logits for ``stats`` from ``label_logprob`` on the same logits; ``g`` float32 of the rows' shape.
     ``out`` may be the logits themselves."""
     lib = _lib.load()
-    d, rows = _logits(logits)
-    _labels(labels, logits)
-    _per_row(stats, (rows, 2), "stats"), _per_row(g, labels.shape, "g")
-    out = _dlogits(logits, out)
+    d, rows, shape = _logits(logits, labels)
+    _per_row(stats, (rows, 2), labels, "stats"), _per_row(g, shape, labels, "g")
+    out, od = _dlogits(logits, d, out)
     if rows:
-        _lib.check(lib.dp_label_logprob_bwd(ctypes.byref(d), _p(labels), _p(stats), _p(g), ctypes.byref(_logits(out, "out")[0]),
+        _lib.check(lib.dp_label_logprob_bwd(ctypes.byref(d), labels.data_ptr(), stats.data_ptr(), g.data_ptr(), ctypes.byref(od),
                                             _stream()), "dp_label_logprob_bwd")
     return out
 
@@ -388,20 +409,19 @@ def preference_loss(logits, labels, cu_seqlens, ref_logp, beta, upstream, label_
     loss = -(1 - label_smoothing) log sigmoid(h) - label_smoothing log sigmoid(-h);
     dlogits = upstream * d sum(loss) / d logits (``out`` may be the logits themselves)."""
     lib = _lib.load()
-    d, rows = _logits(logits)
+    d, rows, _ = _logits(logits, labels)
     if logits.dim() != 2:
         raise ValueError("`logits` must be (R, V): the sequences lie one after the other")
-    _labels(labels, logits)
-    _chk(cu_seqlens, torch.int32, "cu_seqlens"), _here(cu_seqlens, "cu_seqlens")
+    _chk(cu_seqlens, torch.int32, "cu_seqlens"), _beside(cu_seqlens, labels, "cu_seqlens")
     if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1 or cu_seqlens.shape[0] % 2 != 1:
         raise ValueError("`cu_seqlens` must be (2 * pairs + 1,), got %s" % (tuple(cu_seqlens.shape),))
     P = cu_seqlens.shape[0] // 2
-    _per_row(ref_logp, (2 * P,), "ref_logp")
+    _per_row(ref_logp, (2 * P,), labels, "ref_logp")
     if not 0.0 <= label_smoothing <= 1.0:
         raise ValueError("`label_smoothing` must be in [0, 1], got %r" % (label_smoothing,))
     loss = torch.empty((P,), dtype=torch.float32, device=logits.device)
-    seq_logp = torch.empty((2 * P,), dtype=torch.float32, device=logits.device)
-    dlogits = _dlogits(logits, out) if want_grad else None
+    seq_logp = loss.new_empty((2 * P,))
+    dlogits, od = _dlogits(logits, d, out) if want_grad else (None, None)
     if rows == 0 or P == 0:          # nothing that a kernel would read: sums of nothing
         seq_logp.zero_()
         if P:
@@ -409,10 +429,10 @@ def preference_loss(logits, labels, cu_seqlens, ref_logp, beta, upstream, label_
             loss.copy_(torch.nn.functional.softplus(-h) + float(label_smoothing) * h)
         return loss, (dlogits.zero_() if want_grad else None), seq_logp
     work = _logits_workspace(_lib.DP_PREFERENCE, d, logits.device)
-    dd = ctypes.byref(_logits(dlogits, "out")[0]) if want_grad else None
-    _lib.check(lib.dp_preference_loss(ctypes.byref(d), _p(labels), _p(cu_seqlens), P, _p(ref_logp), float(beta), float(upstream),
-                                      float(label_smoothing), 1 if average else 0, _p(loss), _p(seq_logp), dd, _p(work),
-                                      _stream()), "dp_preference_loss")
+    _lib.check(lib.dp_preference_loss(ctypes.byref(d), labels.data_ptr(), cu_seqlens.data_ptr(), P, _ptr(ref_logp), float(beta),
+                                      float(upstream), float(label_smoothing), 1 if average else 0, loss.data_ptr(),
+                                      seq_logp.data_ptr(), ctypes.byref(od) if want_grad else None, _ptr(work), _stream()),
+               "dp_preference_loss")
     return loss, dlogits, seq_logp
 
 
@@ -427,27 +447,26 @@ def policy_loss(logits, labels, old_logp, advantage, clip_low, clip_high, upstre
     dlogits = upstream * d sum(weight * loss) / d logits.  ``old_logp``, ``advantage``, ``ref_logp``, ``weight``: float32 of the
     rows' shape.  ``want_entropy`` None: if entropy_coef is not 0.  ``out`` may be the logits themselves."""
     lib = _lib.load()
-    d, rows = _logits(logits)
-    _labels(labels, logits)
+    d, rows, shape = _logits(logits, labels)
     for name, t in (("old_logp", old_logp), ("advantage", advantage), ("ref_logp", ref_logp), ("weight", weight)):
         if t is None and name in ("old_logp", "advantage"):
             raise TypeError("`%s` is needed" % name)
-        _per_row(t, labels.shape, name)
+        _per_row(t, shape, labels, name)
     if not (0.0 <= clip_low <= 1.0 and clip_high >= 0.0):
         raise ValueError("need 0 <= clip_low <= 1 and clip_high >= 0, got %r, %r" % (clip_low, clip_high))
     if kl_coef != 0.0 and ref_logp is None:
         raise ValueError("`kl_coef` needs `ref_logp`")
     want_entropy = entropy_coef != 0.0 if want_entropy is None else want_entropy
-    loss = torch.empty(labels.shape, dtype=torch.float32, device=logits.device)
-    logp = torch.empty_like(loss)
-    entropy = torch.empty_like(loss) if want_entropy else None
-    dlogits = _dlogits(logits, out) if want_grad else None
+    loss, logp = torch.empty_like(old_logp), torch.empty_like(old_logp)
+    entropy = torch.empty_like(old_logp) if want_entropy else None
+    dlogits, od = _dlogits(logits, d, out) if want_grad else (None, None)
     if rows:
         cfg = _lib.DpPolicyCfg(float(clip_low), float(clip_high), float(kl_coef), float(entropy_coef), float(upstream))
         work = _logits_workspace(_lib.DP_POLICY, d, logits.device)
-        dd = ctypes.byref(_logits(dlogits, "out")[0]) if want_grad else None
-        _lib.check(lib.dp_policy_loss(ctypes.byref(cfg), ctypes.byref(d), _p(labels), _p(old_logp), _p(advantage), _p(ref_logp),
-                                      _p(weight), _p(loss), _p(logp), _p(entropy), dd, _p(work), _stream()), "dp_policy_loss")
+        _lib.check(lib.dp_policy_loss(ctypes.byref(cfg), ctypes.byref(d), labels.data_ptr(), old_logp.data_ptr(),
+                                      advantage.data_ptr(), _ptr(ref_logp), _ptr(weight), loss.data_ptr(), logp.data_ptr(),
+                                      _ptr(entropy), ctypes.byref(od) if want_grad else None, _ptr(work), _stream()),
+                   "dp_policy_loss")
     return loss, dlogits, logp, entropy
 
 

@@ -82,6 +82,7 @@ class AdamW(object):
         self._table = (_lib.DpAdamwTensor * count)()
         self._rows = np.frombuffer(self._table, dtype=np.dtype(_lib.DpAdamwTensor))     # the same memory, a column at a time
         self._numel = np.array([p.numel() for p in self.params], dtype=np.int64)
+        self._shapes, self._devices = [p.shape for p in self.params], {self.params[0].get_device()}
         self._rows["at"] = self.offsets
         self._rows["lr"] = _per_tensor(lr, count, "lr")
         self._rows["weight_decay"] = _per_tensor(weight_decay, count, "weight_decay")
@@ -99,29 +100,31 @@ class AdamW(object):
         return self._steps if self._counter is None else int(self._counter)
 
     def _grads(self, grads):
+        """Columns of the table: (pointers, element types, element counts)."""
         grads = [p.grad for p in self.params] if grads is None else list(grads)
         if len(grads) != len(self.params):
             raise ValueError("`grads` must have one entry for each of the %d tensors, got %d" % (len(self.params), len(grads)))
-        types = ops.ELEMENT_TYPES
-        pointers, kinds = [], []
         numel = self._numel
-        for k, (g, p) in enumerate(zip(grads, self.params)):
-            if g is None:                                  # no gradient: the tensor and its moments stay
-                if numel is self._numel:
-                    numel = numel.copy()
-                numel[k] = 0
-                pointers.append(0)
-                kinds.append(0)
-                continue
-            kind = types.get(g.dtype) if isinstance(g, torch.Tensor) else None
-            if kind is None or not g.is_contiguous() or g.device != p.device:
+        missing = [k for k, g in enumerate(grads) if g is None]
+        if missing:                                        # no gradient: the tensor and its moments stay
+            numel = numel.copy()
+            numel[missing] = 0
+            grads = [self.params[k] if g is None else g for k, g in enumerate(grads)]
+        try:
+            good = ([g.shape for g in grads] == self._shapes and all([g.is_contiguous() for g in grads])
+                    and {g.get_device() for g in grads} == self._devices)
+            types = {g.dtype for g in grads}
+            kinds = [ops.ELEMENT_TYPES[g.dtype] for g in grads] if len(types) > 1 else ops.ELEMENT_TYPES[types.pop()]
+        except (AttributeError, KeyError):
+            good = False
+        if not good:                                       # which one, and why
+            for k, (g, p) in enumerate(zip(grads, self.params)):
                 self._check(g, "grads[%d]" % k)
-                raise ValueError("`grads[%d]` is on %s, its parameter on %s" % (k, g.device, p.device))
-            if g.shape != p.shape:
-                raise ValueError("`grads[%d]` has the shape %s, its parameter %s" % (k, tuple(g.shape), tuple(p.shape)))
-            pointers.append(g.data_ptr())
-            kinds.append(kind)
-        return pointers, kinds, numel
+                if g.shape != p.shape:
+                    raise ValueError("`grads[%d]` has the shape %s, its parameter %s" % (k, tuple(g.shape), tuple(p.shape)))
+                if g.device != p.device:
+                    raise ValueError("`grads[%d]` is on %s, its parameter on %s" % (k, g.device, p.device))
+        return [g.data_ptr() for g in grads], kinds, numel
 
     @torch.no_grad()
     def step(self, grads=None, lr=None):
@@ -131,8 +134,7 @@ class AdamW(object):
         lib = _lib.load()
         rows = self._rows
         pointers, kinds, numel = self._grads(grads)
-        for p in (self.params[0], self.exp_avg, self.exp_avg_sq):
-            ops._here(p, "params")
+        ops._here(self.exp_avg, "params")
         if self._counter is None and self.params[0].is_cuda and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamW.step is being captured: the step count would stay what it is (use capturable=True)")
         if lr is not None:
@@ -149,9 +151,10 @@ class AdamW(object):
             if self.max_norm is not None:
                 norm = torch.empty((), dtype=torch.float32, device=dev)
         cfg.step = self._steps + 1
-        _lib.check(lib.dp_adamw_step(ctypes.byref(cfg), self._table, count, ops._p(self.exp_avg), ops._p(self.exp_avg_scale),
-                                     ops._p(self.exp_avg_sq), ops._p(self.exp_avg_sq_scale), ops._p(self._counter),
-                                     ops._p(norm), ops._p(work), ops._stream()), "dp_adamw_step")
+        ptr = ops._ptr
+        _lib.check(lib.dp_adamw_step(ctypes.byref(cfg), self._table, count, ptr(self.exp_avg), ptr(self.exp_avg_scale),
+                                     ptr(self.exp_avg_sq), ptr(self.exp_avg_sq_scale), ptr(self._counter), ptr(norm), ptr(work),
+                                     ops._stream()), "dp_adamw_step")
         self._steps += 1
         torch.autograd.graph.increment_version(self.params)     # written in place, as autograd has to know
         return norm

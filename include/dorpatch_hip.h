@@ -466,7 +466,8 @@ int dp_policy_loss(const dp_policy_cfg_t *cfg, const dp_logits_t *x, const int64
 
 /* AdamW over many tensors at once.  The table of tensors is HOST memory (copied into the launches: nothing of it is kept):
  * n elements of param and grad (dense; any element alignment; DP_F32 / DP_BF16 / DP_F16 each; n <= 2^34), the place
- * `at` of its part in the states (a multiple of DP_ADAMW_BLOCK, parts padded to a multiple of it and disjoint), lr and weight_decay.  Per element, every operation rounded to fp32:
+ * `at` of its part in the states (a multiple of DP_ADAMW_BLOCK, parts padded to a multiple of it and disjoint), lr and weight_decay.  Per element, in fp32 (the moments with one rounding per operation, so that
+ * their bits do not depend on the machine; the last quotient to 3 units in the last place):
  *   g' = g * clip,  m = beta1 m + (1 - beta1) g',  v = beta2 v + (1 - beta2) g'^2,
  *   param = param (1 - lr weight_decay) - (m / (sqrt(v) / sqrt(1 - beta2^t) + eps)) * (lr / (1 - beta1^t)),  then clamped to
  *   [box_low, box_high] if box; rounded to nearest where param is narrower than fp32.

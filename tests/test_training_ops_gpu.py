@@ -654,7 +654,7 @@ def test_c_entries_refuse_what_the_kernels_do_not_take():
     for bad in (dict(data=0), dict(data=x.data_ptr() + 2), dict(dtype=3), dict(rows=0), dict(rows=2 ** 23 + 1), dict(vocab=0), dict(inner=0), dict(row_stride=-8)):
         assert lib.dp_label_logprob(rows(**bad), P(y.data_ptr()), P(o.data_ptr()), None, None, None, ops._stream()) == 1, bad
     assert lib.dp_label_logprob(rows(), None, P(o.data_ptr()), None, None, None, ops._stream()) == 1
-    assert lib.dp_logits_workspace(7, 4, 8, 0) == 0 and lib.dp_logits_workspace(_lib.DP_POLICY, 4, 8, 0) >= 64
+    assert lib.dp_logits_workspace(7, 4, 8, 0) == 0 and lib.dp_logits_workspace(_lib.DP_PREFERENCE, 4, 8, 0) >= 4 * 28
     table = (_lib.DpAdamwTensor * 2)()
     for k in range(2):
         table[k].param, table[k].grad, table[k].n, table[k].at = o.data_ptr() + 64 * k, x.data_ptr(), 16, 128 * k
