@@ -280,7 +280,11 @@ class DorPatch(object):
         ``tape_tabs`` (micro-batches whose activations one backward may draw from, default: what fits in half of the free
         HBM, at most 8), ``backward_ladder`` (batch sizes the selected-sample backward may use), ``placement``
         (EXTENSION, not in the reference: e.g. ``dorpatch_amd.placement.RandomAffine()`` — every EOT sample sees the
-        patch under its own random affine placement; ``None`` = the reference's identity placement).
+        patch under its own random affine placement; ``None`` = the reference's identity placement), ``update``
+        (EXTENSION, not in the reference: ``"adamw"`` — pattern and mask of every image follow their gradients through
+        ``dorpatch_amd.optim.AdamW`` without decay, lr as the schedule has it, clamped to [clip_min, clip_max], moments
+        from zero in each stage; ``"sign"``, the default: the reference's signed update, ``attack.py:333-342``),
+        ``adamw`` (a dict of that optimiser's ``betas``, ``eps``, ``state_bits``, ``seed``).
         """
         run = HotLoop(self, model, x, patch_budget, n_classes, save_dir, batch_id, y, targeted, lr,
                       confidence, clip_min, clip_max, max_iterations, basic_unit, selection, dropout,
@@ -536,6 +540,14 @@ class HotLoop(object):
         # EXTENSION (dorpatch_amd/placement.py; absent from the reference, which places the patch at identity):
         # an object with .draw(rng, S, H, W) -> (S,2,3) output->source pixel maps, one draw per image per step
         self.placement = extras.get("placement", None)
+        # EXTENSION (dorpatch_amd/optim.py): how pattern and mask follow their gradients
+        self.update = extras.get("update", "sign")
+        if self.update not in ("sign", "adamw"):
+            raise ValueError("update must be 'sign' or 'adamw' (got %r)" % (self.update,))
+        self._adamw_args = dict(extras.get("adamw", {}))
+        if not set(self._adamw_args) <= {"betas", "eps", "state_bits", "seed"}:
+            raise ValueError("adamw takes betas, eps, state_bits, seed (got %s)" % sorted(self._adamw_args))
+        self._adamw = None
 
         self.net, self.norm = _unwrap_model(model)
         self.dn = _dp_norm(self.norm)
@@ -976,16 +988,29 @@ class HotLoop(object):
 
         # --- a-2 backward + a-5/a-6 gradients + signed update (attack.py:247, 333-342)
         ph.mark("dp:project_update")
-        ops.project_update(
+        adamw = self.update == "adamw"
+        grads = ops.project_update(
             self.x, self.adv_x, self.lv_x, self.g_adv, scale, self._dev_f32(structured_pre),
             self.adv_pattern, self.adv_mask, stage=stage, lr=self._dev_f32(lr_now),
             coeff_gl=self._dev_f32(coeff_pre), cell_sumsq=cell, win_sum=wsum, unit=self.unit,
             win=self.win, density=self.density, clip_min=self.clip_min, clip_max=self.clip_max,
             save_best=self._dev_i32(save_best), best_pattern=self.best_pattern,
-            best_mask=self.best_mask, do_update=True)
+            best_mask=self.best_mask, do_update=not adamw, want_grads=adamw)
+        if adamw:
+            self._adamw_update(*grads, lr_now)
         ph.mark(None)
         self.samples_done += B * S
         return any(st.active for st in self.img)
+
+    def _adamw_update(self, g_pattern, g_mask, lr):
+        """AdamW on every image's pattern (stage 0: and mask), each with its image's lr (0: finished).  The gradient of a mask cell
+        that is all 0 is NaN, which the signed update freezes at 0 (sign(NaN) = 0): here it counts as 0 and the cell stays."""
+        learned = [(self.adv_pattern, g_pattern)] + ([(self.adv_mask, torch.nan_to_num(g_mask, nan=0.0))] if self.stage == 0 else [])
+        if self._adamw is None or self._adamw[0] != self.stage:
+            from . import optim
+            self._adamw = (self.stage, optim.AdamW([p[b] for p, _ in learned for b in range(self.B)], weight_decay=0.0,
+                                                   box=(self.clip_min, self.clip_max), **self._adamw_args))
+        self._adamw[1].step([g[b] for _, g in learned for b in range(self.B)], lr=[float(v) for v in lr] * len(learned))
 
     def _draw_checksum(self):
         """A float-exact fingerprint of this step's draws — the mask indices, the second (``dual``) index set and the

@@ -1,0 +1,72 @@
+"""DorPatch.generate(update="adamw") (extension: dorpatch_amd/optim.py on pattern and mask) against the update's formula in 64 bits on
+the gradients that the step reports.  test_adamw_attack_emu.py runs the same on the CPU emulation."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from dorpatch_amd.attack import DorPatch  # noqa: E402
+from dorpatch_amd.utils import NormModel, get_normalize  # noqa: E402
+from oracle import toy_models  # noqa: E402
+
+DEV = "cuda:0"
+U = 2.0 ** -24
+
+
+def _run(tmp_path, monkeypatch, seen, n_it=4, B=2, **extra):
+    monkeypatch.chdir(tmp_path)
+    H, S = 56, 4
+    model = NormModel(toy_models.make_toy(gain=2.0), get_normalize("imagenet", "resnetv2")).to(DEV)
+    g = torch.Generator().manual_seed(5)
+    x = torch.rand(B, 3, H, H, generator=g).to(DEV)
+    y = torch.tensor([1, 2][:B]).to(DEV)
+    atk = DorPatch(verbose=False)
+
+    def hook(d):
+        seen.append({k: (v.detach().cpu().clone() if torch.is_tensor(v) else np.array(v)) for k, v in d.items()
+                     if k in ("stage", "i", "grad_pattern", "grad_mask", "mask", "pattern", "lr")})
+    return atk.generate(model, x, 0.12, 10, "res/cfg/sub", 0, y=y, targeted=True, lr=0.01, sampling_size=S, max_iterations=n_it,
+                        init_mask=torch.rand(B, 1, H, H, generator=g) * (torch.arange(H) >= 7), init_pattern=torch.rand(B, 3, H, H, generator=g),
+                        rngs=[np.random.RandomState(b) for b in range(B)], step_hook=hook, **extra)
+
+
+def test_pattern_and_mask_follow_adamw(tmp_path, monkeypatch):
+    seen = []
+    _run(tmp_path, monkeypatch, seen, update="adamw", adamw=dict(betas=(0.8, 0.95)))
+    assert [int(d["stage"]) for d in seen] == [0] * 4 + [1] * 4
+    for name, learned_in in (("pattern", (0, 1)), ("mask", (0,))):
+        for stage in (0, 1):
+            steps = [d for d in seen if d["stage"] == stage]
+            m = v = torch.zeros_like(steps[0][name]).double()
+            for t, (d, after) in enumerate(zip(steps, steps[1:]), 1):
+                if stage not in learned_in:
+                    assert torch.equal(d[name], after[name])
+                    continue
+                g = torch.nan_to_num(d["grad_" + name].double(), nan=0.0)
+                m, v = 0.8 * m + 0.2 * g, 0.95 * v + 0.05 * g * g
+                lr = torch.from_numpy(d["lr"]).double().view(-1, 1, 1, 1)
+                change = lr * (m / (1 - 0.8 ** t)) / ((v / (1 - 0.95 ** t)).sqrt() + 1e-8)
+                want = (d[name].double() - change).clamp(0, 1)
+                # the moments round once per operation (3 a step), root, quotient and rate 6 times, the difference once
+                assert ((after[name].double() - want).abs() <= 2 * U * (want.abs() + d[name].abs()) + (3 * t + 8) * U * (change.abs() + lr)).all(), (name, stage, t)
+                frozen = (d[name] == 0) & (d["grad_" + name].isnan() | (d["grad_" + name] == 0)) & (m == 0)
+                assert (after[name][frozen] == 0).all()
+    # the mask's first columns start at 0: their cells' gradient is NaN, and they stay
+    assert seen[0]["grad_mask"][..., :7].isnan().any() and (seen[3]["mask"][..., :7][seen[0]["grad_mask"][..., :7].isnan()] == 0).all()
+    assert all(torch.isfinite(d["pattern"]).all() and torch.isfinite(d["mask"]).all() for d in seen)
+
+
+def test_runs_repeat_bit_for_bit_with_8_bit_moments(tmp_path, monkeypatch):
+    outs = []
+    for k in range(2):
+        (tmp_path / str(k)).mkdir()
+        outs.append(_run(tmp_path / str(k), monkeypatch, [], update="adamw", adamw=dict(state_bits=8, seed=11)))
+    assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])
+
+
+def test_unknown_updates_are_refused(tmp_path, monkeypatch):
+    with pytest.raises(ValueError, match="update"):
+        _run(tmp_path, monkeypatch, [], update="sgd")
+    with pytest.raises(ValueError, match="adamw takes"):
+        _run(tmp_path, monkeypatch, [], update="adamw", adamw=dict(lr=1.0))

@@ -677,3 +677,67 @@ def test_c_entries_refuse_what_the_kernels_do_not_take():
     assert step() == 1
     cfg.state_bits, cfg.max_norm = 32, 1.0          # no counter
     assert step() == 1
+
+
+# ---------------------------------------------------------------- together
+def adamw_reference(state, p, g, t, lr, decay, clip):
+    m, v = state
+    p, state[0], state[1] = adamw64(p, g, m, v, t, lr, (0.9, 0.999), 1e-8, decay, clip)
+    return p
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_steps_of_a_policy_and_a_preference_together(bits):
+    """A linear model over 60 categories: three steps of the policy loss, then three of the preference loss against the model
+    before, each with the gradient through the product and a clipped AdamW step: the parameters as in 64 bits throughout.
+
+    32 bits: a step's gradient is off by about 3e-5 of itself (check_grad's 2e-5 and the product's roundings); Adam's first steps
+    scale every element to about lr, an element of the gradient much under the others moves by lr times its own relative error,
+    so that few elements may be off more than 1e-3 lr and none more than 2 lr a step.  8 bits: the first step is the same; what is kept after
+    it is a code off by at most an eighth (m) and an eighth (v, so a sixteenth in its root): a step differs by less than a third."""
+    V, d, R, lr = 60, 16, 24, 1e-2
+    w = rand(V, d, seed=1, scale=0.3)
+    bias = rand(V, seed=2, scale=0.1)
+    x = rand(R, d, seed=3)
+    y = make_labels((R,), V, seed=4)
+    adv = rand(R, seed=5)
+    cu = [0, 5, 9, 16, R]
+    params = [w.clone().to(DEV), bias.clone().to(DEV)]
+    opt = optim.AdamW(params, lr=lr, weight_decay=[0.1, 0.0], state_bits=bits, max_norm=0.5, seed=9)
+    p64 = [w.double(), bias.double()]
+    states = [[torch.zeros_like(p), torch.zeros_like(p)] for p in p64]
+    xd, yd = x.to(DEV), y.to(DEV)
+    old = ref = None
+    for t in range(1, 7):
+        logits = (xd @ params[0].t() + params[1]).contiguous()
+        l64 = x.double() @ p64[0].t() + p64[1]
+        if t <= 3:
+            if old is None:
+                old, old64 = ops.label_logprob(logits, yd)[0], softmax64(l64, y)[1]
+            loss, dl, _, _ = ops.policy_loss(logits, yd, old, adv.to(DEV), 0.2, 0.2, 1.0 / R, entropy_coef=0.01, out=logits)
+            dl64 = policy64(l64, y, old64, adv, 0.2, 0.2, 1.0 / R, None, 0.0, 0.01, None)[1]
+        else:
+            if ref is None:
+                lp, lp64 = ops.label_logprob(logits, yd)[0], softmax64(l64, y)[1]
+                ref = torch.stack([lp[a:b].sum() for a, b in zip(cu[:-1], cu[1:])])
+                ref64 = torch.stack([lp64[a:b].sum() for a, b in zip(cu[:-1], cu[1:])])
+            loss, dl, _ = ops.preference_loss(logits, yd, torch.tensor(cu, dtype=torch.int32).to(DEV), ref, 0.5, 0.5)
+            dl64 = preference64(l64, y, cu, ref64, 0.5, 0.0, False, 0.5)[1]
+        norm = opt.step([(dl.t() @ xd).contiguous(), dl.sum(0)])
+        g64 = [dl64.t() @ x.double(), dl64.sum(0)]
+        n64 = math.sqrt(sum(float(g.square().sum()) for g in g64))
+        clip = min(1.0, 0.5 / (n64 + 1e-6))
+        for k, decay in enumerate((0.1, 0.0)):
+            p64[k] = adamw_reference(states[k], p64[k], g64[k], t, lr, decay, clip)
+        if bits == 32:
+            assert abs(float(norm) / n64 - 1) <= 1e-3
+        for p, q in zip(params, p64):
+            err = (p.cpu().double() - q).abs()
+            if bits == 32:
+                assert err.max() <= 2 * lr * t and (err > 1e-3 * lr * t).float().mean() <= 0.02, (t, err.max())
+            else:
+                assert err.mean() <= lr / 3 * t and err.max() <= 2 * lr * t, (t, err.mean(), err.max())
+        if bits == 8 and t == 1:
+            for p, q in zip(params, p64):
+                assert ((p.cpu().double() - q).abs() <= 1e-3 * lr).float().mean() >= 0.98
+    assert opt.steps == 6 and torch.isfinite(loss).all()
