@@ -27,8 +27,8 @@
 // families share (macros, reductions, the debug knobs) and the list of family files below; the product build
 // (dorpatch_amd/build.py) compiles it six times IN PARALLEL with -DDP_PART=1..6 — 1: apply.inc + update.inc (the DorPatch
 // arithmetic), gn.inc, stem.inc; 2: conv3x3.inc (direct 3x3, stride 1); 3: conv1x1.inc; 4: conv3x3_wino.inc; 5: conv3x3s2.inc
-// (stride-2 3x3 and its input gradient); 6: logits.inc + adamw.inc (losses and optimiser of a training step) — and links the objects into the one libdorpatch_hip.so; a kernel, its launcher and
-// its extern "C" entry point live in the same file.  DP_PART = 0 (the default: tools/kbench's white-box include, the host
+// (stride-2 3x3 and its input gradient); 6: logits.inc + adamw.inc (losses and optimiser of a training step) — and links
+// the objects into the one libdorpatch_hip.so; a kernel, its launcher and its extern "C" entry point live in the same file.  DP_PART = 0 (the default: tools/kbench's white-box include, the host
 // emulation of tests/hipemu) is the whole library in one unit.
 #ifndef DP_PART
 #define DP_PART 0

@@ -2,7 +2,7 @@
 
 Beside the signed update of the patch (``ops.project_update``): for what is trained by its gradient's moments — the patterns
 and masks of many images (``DorPatch.generate(update="adamw")``), or a classifier's own weights.  One step is one launch for
-up to 72 tensors, plus two small ones where the gradients are clipped by their global norm; it never synchronises.
+up to 98 tensors, plus two small ones where the gradients are clipped by their global norm; it never synchronises.
 """
 import ctypes
 
@@ -12,14 +12,17 @@ import torch
 from . import _lib, ops
 
 BLOCK = _lib.DP_ADAMW_BLOCK
+# for map() over a hundred tensors a step
+_DTYPE, _SHAPE, _NUMEL = torch.Tensor.dtype.__get__, torch.Tensor.shape.__get__, torch.Tensor.numel
+_DENSE, _DEVICE, _POINTER = torch.Tensor.is_contiguous, torch.Tensor.get_device, torch.Tensor.data_ptr
 
 
 def _per_tensor(value, count, name):
     values = [float(value)] * count if not isinstance(value, (list, tuple)) else [float(v) for v in value]
     if len(values) != count:
         raise ValueError("`%s` must be a number or one for each of the %d tensors, got %d" % (name, count, len(values)))
-    if not all(v >= 0.0 for v in values):
-        raise ValueError("`%s` must be >= 0" % name)
+    if not all(0.0 <= v < float("inf") for v in values):
+        raise ValueError("`%s` must be finite and >= 0" % name)
     return values
 
 
@@ -61,6 +64,7 @@ class AdamW(object):
             raise ValueError("`box` must be (low, high) or None, got %r" % (box,))
         count = len(self.params)
         self.lr = lr
+        self._versioned = [p for p in self.params if not p.is_inference()]
         self.offsets, at = [], 0
         for p in self.params:
             self.offsets.append(at)
@@ -83,6 +87,7 @@ class AdamW(object):
         self._rows = np.frombuffer(self._table, dtype=np.dtype(_lib.DpAdamwTensor))     # the same memory, a column at a time
         self._numel = np.array([p.numel() for p in self.params], dtype=np.int64)
         self._shapes, self._devices = [p.shape for p in self.params], {self.params[0].get_device()}
+        self._types, self._sizes = [p.dtype for p in self.params], [p.numel() for p in self.params]
         self._rows["at"] = self.offsets
         self._rows["lr"] = _per_tensor(lr, count, "lr")
         self._rows["weight_decay"] = _per_tensor(weight_decay, count, "weight_decay")
@@ -99,6 +104,13 @@ class AdamW(object):
         """Steps taken (reads the device where the counter lives there)."""
         return self._steps if self._counter is None else int(self._counter)
 
+    def _same(self):
+        """The launch writes where the parameters lie now: one given other data since (``p.data = ...``) must fit the states."""
+        ps = self.params
+        if (list(map(_DTYPE, ps)) != self._types or list(map(_NUMEL, ps)) != self._sizes
+                or not all(map(_DENSE, ps)) or set(map(_DEVICE, ps)) != self._devices):
+            raise ValueError("`params` have other sizes, types or strides, or another device, than the optimiser was made for")
+
     def _grads(self, grads):
         """Columns of the table: (pointers, element types, element counts)."""
         grads = [p.grad for p in self.params] if grads is None else list(grads)
@@ -111,11 +123,11 @@ class AdamW(object):
             numel[missing] = 0
             grads = [self.params[k] if g is None else g for k, g in enumerate(grads)]
         try:
-            good = ([g.shape for g in grads] == self._shapes and all([g.is_contiguous() for g in grads])
-                    and {g.get_device() for g in grads} == self._devices)
-            types = {g.dtype for g in grads}
+            good = (list(map(_SHAPE, grads)) == self._shapes and all(map(_DENSE, grads))
+                    and set(map(_DEVICE, grads)) == self._devices)
+            types = set(map(_DTYPE, grads))
             kinds = [ops.ELEMENT_TYPES[g.dtype] for g in grads] if len(types) > 1 else ops.ELEMENT_TYPES[types.pop()]
-        except (AttributeError, KeyError):
+        except (TypeError, KeyError):
             good = False
         if not good:                                       # which one, and why
             for k, (g, p) in enumerate(zip(grads, self.params)):
@@ -124,15 +136,15 @@ class AdamW(object):
                     raise ValueError("`grads[%d]` has the shape %s, its parameter %s" % (k, tuple(g.shape), tuple(p.shape)))
                 if g.device != p.device:
                     raise ValueError("`grads[%d]` is on %s, its parameter on %s" % (k, g.device, p.device))
-        return [g.data_ptr() for g in grads], kinds, numel
+        return list(map(_POINTER, grads)), kinds, numel
 
-    @torch.no_grad()
     def step(self, grads=None, lr=None):
         """One step from ``grads`` (a list; None: every parameter's ``.grad``; an entry None: that tensor stays), in place.
         ``lr``: a number or one for each tensor, for this and the next steps.  Returns the global gradient norm before clipping
         (a 0-dim float32 tensor) where ``max_norm`` is set, else None."""
         lib = _lib.load()
         rows = self._rows
+        self._same()
         pointers, kinds, numel = self._grads(grads)
         ops._here(self.exp_avg, "params")
         if self._counter is None and self.params[0].is_cuda and torch.cuda.is_current_stream_capturing():
@@ -140,8 +152,8 @@ class AdamW(object):
         if lr is not None:
             rows["lr"] = _per_tensor(lr, len(self.params), "lr")
             self.lr = lr
-        rows["param"] = [p.data_ptr() for p in self.params]
-        rows["grad"], rows["grad_dtype"], rows["n"] = pointers, kinds, numel
+        rows["param"], rows["grad"] = list(map(_POINTER, self.params)), pointers
+        rows["grad_dtype"], rows["n"] = kinds, numel
         cfg, count = self._cfg, len(self.params)
         norm = work = None
         dev = self.params[0].device
@@ -156,7 +168,7 @@ class AdamW(object):
                                      ptr(self.exp_avg_sq), ptr(self.exp_avg_sq_scale), ptr(self._counter), ptr(norm), ptr(work),
                                      ops._stream()), "dp_adamw_step")
         self._steps += 1
-        torch.autograd.graph.increment_version(self.params)     # written in place, as autograd has to know
+        torch.autograd.graph.increment_version(self._versioned)     # written in place, as autograd has to know
         return norm
 
     def moments(self, k):

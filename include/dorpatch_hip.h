@@ -410,7 +410,8 @@ int dp_subsample2_add(const float *dy, int64_t NC, int H, int W, float *g, dp_st
  *
  * Rows of logits: row r of `rows` lies at  data + (r / inner) * outer_stride + (r % inner) * row_stride  elements (strides >= 0;
  * a dense (R, V) tensor: inner = R, row_stride = V; the slice x[:, :-1] of a (B, T, V) tensor: inner = T - 1, row_stride = V,
- * outer_stride = T * V), its `vocab` elements side by side; any element alignment.  rows <= 2^23, vocab <= 2^30.
+ * outer_stride = T * V), its `vocab` elements side by side; any element alignment.  rows <= 2^23, vocab <= 2^30,
+ * rows * ceil(bytes of a row / 16384) < 2^24.
  * labels (rows) int64.  A label < 0 marks a row that counts for nothing (a prompt, padding): its logits are not read, its
  * outputs and its gradient are 0 whatever is in it.  So does a row whose logits are all -inf.  A label >= vocab gives NaN in
  * the row's outputs and gradient, and no access.  Single logits may be -inf (not allowed: probability 0).
@@ -466,8 +467,9 @@ int dp_policy_loss(const dp_policy_cfg_t *cfg, const dp_logits_t *x, const int64
 
 /* AdamW over many tensors at once.  The table of tensors is HOST memory (copied into the launches: nothing of it is kept):
  * n elements of param and grad (dense; any element alignment; DP_F32 / DP_BF16 / DP_F16 each; n <= 2^34), the place
- * `at` of its part in the states (a multiple of DP_ADAMW_BLOCK, parts padded to a multiple of it and disjoint), lr and weight_decay.  Per element, in fp32 (the moments with one rounding per operation, so that
- * their bits do not depend on the machine; the last quotient to 3 units in the last place):
+ * `at` of its part in the states (a multiple of DP_ADAMW_BLOCK, parts padded to a multiple of it and disjoint), lr and
+ * weight_decay.  Per element, in fp32 (the moments with one rounding per operation, so that their bits do not depend on the
+ * machine; the last quotient to 3 units in the last place, for v of 2^-126 and up):
  *   g' = g * clip,  m = beta1 m + (1 - beta1) g',  v = beta2 v + (1 - beta2) g'^2,
  *   param = param (1 - lr weight_decay) - (m / (sqrt(v) / sqrt(1 - beta2^t) + eps)) * (lr / (1 - beta1^t)),  then clamped to
  *   [box_low, box_high] if box; rounded to nearest where param is narrower than fp32.

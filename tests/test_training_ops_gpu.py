@@ -155,6 +155,36 @@ def test_banned_entries_and_strange_rows(V, dtype):
     assert torch.isnan(logp[8]) and torch.isnan(d[8]).all()
 
 
+@pytest.mark.parametrize("R,V", [(3, 7), (3, 2000), (70, 5000), (2, 40000)])
+def test_rows_of_nan_alone_count(R, V):
+    """Short rows, one workgroup a row, rows cut into slices; the fused and the two-pass policy loss."""
+    for dtype in sorted(DTYPES):
+        x = make_logits((R, V), dtype)
+        x[1] = NAN
+        y = torch.ones(R, dtype=torch.int64)
+        xd, yd, one = x.to(DEV), y.to(DEV), torch.ones(R).to(DEV)
+        logp, ent, stats = ops.label_logprob(xd, yd, want_entropy=True)
+        d = ops.label_logprob_bwd(xd, yd, stats, one)
+        loss, dp, lp, h = ops.policy_loss(xd, yd, one, one, 0.2, 0.2, 1.0, entropy_coef=0.1)
+        for t in (logp, ent, d, loss, dp, lp, h):
+            t = t.cpu()
+            assert torch.isnan(t[1]).all() and torch.isfinite(t[0]).all() and torch.isfinite(t[R - 1 if R > 2 else 0]).all()
+        cu = torch.tensor([0, 2, R], dtype=torch.int32).to(DEV)
+        loss, d, seq = ops.preference_loss(xd, yd, cu, None, 0.1, 1.0)
+        assert torch.isnan(loss).all() and torch.isnan(seq[0]) and torch.isnan(d).all()
+
+
+def test_an_entry_far_above_long_sums():
+    """Lanes that hold sums over 2^28 meet an entry of 2^101: nothing is left of them, and no 0 * infinity."""
+    x = torch.full((1, 16384), 16.0)
+    x[0, :1024] = 0.0
+    x[0, 5000] = 2.0 ** 101
+    y, one = torch.tensor([5000]).to(DEV), torch.ones(1).to(DEV)
+    for logp, ent in (ops.label_logprob(x.to(DEV), y, want_entropy=True)[:2],
+                      ops.policy_loss(x.to(DEV), y, one, one, 0.2, 0.2, 1.0, entropy_coef=0.1)[2:]):
+        assert logp[0] == 0 and ent[0] == 0
+
+
 # ---------------------------------------------------------------- preference loss
 def preference64(x, y, cu, ref, beta, smoothing, average, upstream):
     """(loss, dlogits, seq_logp, g) by autograd in 64 bits."""
@@ -218,6 +248,22 @@ def test_preference_loss_far_apart():
         assert torch.isfinite(loss).all() and torch.isfinite(d).all()
         assert ((loss.cpu().double() - wl).abs() <= 2 * LOG_S + 2 * U * wl.abs()).all()
         check_grad(d, wd, g, softmax64(x, y)[0], y, "fp32", g_err=2 * LOG_S + 2 * U)
+
+
+def test_preference_loss_with_a_banned_label():
+    """An impossible sequence: h is infinite, the loss 0 and without gradient, or infinite with the whole slope."""
+    x = make_logits((2, 60), "fp32")
+    x[1, 5] = -INF
+    y = torch.tensor([3, 5])
+    for first, second, want, slope in ((0, 1, 0.0, 0.0), (1, 0, INF, 0.5)):
+        xs, ys = x[[first, second]], y[[first, second]]
+        loss, d, seq = ops.preference_loss(xs.to(DEV), ys.to(DEV), torch.tensor([0, 1, 2], dtype=torch.int32).to(DEV), None, 0.5, 1.0)
+        assert loss[0] == want and seq[second] == -INF and torch.isfinite(seq[first])
+        p = softmax64(xs, ys)[0]
+        g = torch.tensor([slope, -slope])
+        check_grad(d, g[:, None] * (p - onehot(ys, 60)), -g, p, ys, "fp32")
+    loss, _, _ = ops.preference_loss(x.to(DEV), y.to(DEV), torch.tensor([0, 1, 2], dtype=torch.int32).to(DEV), None, 0.5, 1.0, label_smoothing=0.1)
+    assert loss[0] == INF                           # with a weight of its own the other term counts
 
 
 def test_preference_loss_of_nothing():
@@ -637,7 +683,24 @@ def test_adamw_refuses_what_it_does_not_take():
     refused(ValueError, opt.step, [torch.zeros(20).to(DEV)[::2]])
     refused(ValueError, opt.load_state, torch.zeros(5).to(DEV), torch.zeros(5).to(DEV), 1)
     refused(ValueError, opt.load_state, opt.exp_avg, opt.exp_avg_sq, -1)
+    refused(ValueError, optim.AdamW, [p], lr=INF)
+    refused(ValueError, opt.step, [p.clone()], lr=NAN)
     assert opt.steps == 0 and (p == 0).all()
+
+
+def test_adamw_refuses_parameters_that_have_changed():
+    """`.data` given another type, size or stride since: the states no longer fit, and nothing is written."""
+    for change in (lambda t: t.half(), lambda t: t[:5].clone(), lambda t: torch.zeros(20).to(DEV)[::2], lambda t: torch.zeros(1).to(DEV).expand(10)):
+        p = torch.nn.Parameter(torch.zeros(10).to(DEV))
+        opt = optim.AdamW([p])
+        p.data = change(p.data)
+        refused(ValueError, opt.step, [torch.ones(10).to(DEV)])
+        assert (p == 0).all() and opt.steps == 0
+    p = torch.nn.Parameter(torch.zeros(10).to(DEV))
+    opt = optim.AdamW([p], weight_decay=0.0)
+    p.data = torch.ones(10).to(DEV)                 # other data of the same kind: taken where it lies
+    opt.step([torch.ones(10).to(DEV)])
+    assert ((p - (1 - 1e-3)).abs() <= 1e-7).all()
 
 
 def test_c_entries_refuse_what_the_kernels_do_not_take():
