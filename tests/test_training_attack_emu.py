@@ -1,4 +1,4 @@
-"""tests/test_adamw_attack_gpu.py on CPU tensors through the HIP emulation."""
+"""tests/test_training_attack_gpu.py on CPU tensors through the HIP emulation."""
 import importlib.util
 import os
 
@@ -12,7 +12,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 if emu_patch.build_emu.host_compiler() is None:
     pytest.skip("no host clang++ for the HIP emulation build", allow_module_level=True)
 
-_spec = importlib.util.spec_from_file_location("_adamw_attack_on_emu", os.path.join(HERE, "test_adamw_attack_gpu.py"))
+_spec = importlib.util.spec_from_file_location("_training_attack_on_emu", os.path.join(HERE, "test_training_attack_gpu.py"))
 _mod = importlib.util.module_from_spec(_spec)
 _spec.loader.exec_module(_mod)
 _mod.DEV = "cpu"

@@ -1,5 +1,5 @@
 """DorPatch.generate(update="adamw") (extension: dorpatch_amd/optim.py on pattern and mask) against the update's formula in 64 bits on
-the gradients that the step reports.  test_adamw_attack_emu.py runs the same on the CPU emulation."""
+the gradients that the step reports.  test_training_attack_emu.py runs the same on the CPU emulation."""
 import numpy as np
 import pytest
 import torch
