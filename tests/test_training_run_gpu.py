@@ -158,6 +158,26 @@ def test_many_short_rows():
     assert (d.double() - w).abs().max() <= 2e-5
 
 
+def test_rows_of_4_to_6_kb():
+    """A wave a row from 4096 rows on, a workgroup a row below: the same rows both ways, and against 64 bits."""
+    R, V = 4096, 1400
+    x, y = rand(R, V, seed=1, scale=3).to(DEV), torch.randint(0, V, (R,), generator=torch.Generator().manual_seed(2)).to(DEV)
+    x[:, 3] = -float("inf")
+    y[y == 3] = 4
+    y[::9] = -1
+    logp, ent, stats = ops.label_logprob(x, y, want_entropy=True)
+    few, e, st = ops.label_logprob(x[:200], y[:200], want_entropy=True)
+    p = torch.softmax(x.double(), 1)
+    want = torch.log_softmax(x.double(), 1).gather(1, y.clamp(min=0)[:, None])[:, 0] * (y >= 0)
+    h = -torch.xlogy(p, p).sum(1) * (y >= 0)
+    for a, b, n in ((logp, ent, R), (few, e, 200)):
+        assert (a.double() - want[:n]).abs().max() <= 6e-6 and (b.double() - h[:n]).abs().max() <= 6e-6
+    w = (torch.nn.functional.one_hot(y.clamp(min=0), V) - p) * (y >= 0)[:, None]
+    one = torch.ones(R, device=DEV)
+    for d, n in ((ops.label_logprob_bwd(x, y, stats, one), R), (ops.label_logprob_bwd(x[:200], y[:200], st, one[:200]), 200)):
+        assert (d.double() - w[:n]).abs().max() <= 2e-5
+
+
 def test_tensors_of_the_host_are_refused_and_mixed_ones():
     x, y = torch.randn(4, 9, device=DEV), torch.zeros(4, dtype=torch.int64, device=DEV)
     r = torch.zeros(4, device=DEV)
