@@ -69,6 +69,7 @@ class AdamW(object):
         for p in self.params:
             self.offsets.append(at)
             at += -(-p.numel() // BLOCK) * BLOCK
+        at = max(at, BLOCK)                                # (of empty tensors alone too: the kernels take no null states)
         dev = self.params[0].device
         self.state_bits, self.max_norm = state_bits, max_norm
         dtype = torch.float32 if state_bits == 32 else torch.float8_e4m3fn

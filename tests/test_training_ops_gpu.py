@@ -688,6 +688,16 @@ def test_adamw_refuses_what_it_does_not_take():
     assert opt.steps == 0 and (p == 0).all()
 
 
+def test_adamw_of_nothing():
+    e = torch.zeros(0, 3).to(DEV)
+    for bits, max_norm in ((32, None), (8, 1.0)):
+        opt = optim.AdamW([e], state_bits=bits, max_norm=max_norm)
+        norm = opt.step([e.clone()])
+        assert opt.steps == 1 and (norm is None or norm == 0)
+        norm = opt.step([None])
+        assert opt.steps == 2 and (norm is None or norm == 0) and opt.moments(0)[0].shape == (0, 3)
+
+
 def test_adamw_refuses_parameters_that_have_changed():
     """`.data` given another type, size or stride since: the states no longer fit, and nothing is written."""
     for change in (lambda t: t.half(), lambda t: t[:5].clone(), lambda t: torch.zeros(20).to(DEV)[::2], lambda t: torch.zeros(1).to(DEV).expand(10)):
