@@ -49,9 +49,8 @@ PARTS = (1, 2, 3, 4, 5, 6)  # -DDP_PART values: the kernel families of csrc/*.in
 def build_extension(force=False, verbose=False, jobs=None):
     """Compile the HIP kernels + C ABI. Returns the path of the shared library.
 
-    Round 6: one file per kernel family (``csrc/*.inc``), compiled as six translation units
-    (``-DDP_PART=1..6``) by concurrent hipcc processes and linked into the one library — 26 s of wall time instead of 75 on
-    the 8-core build container."""
+    One file per kernel family (``csrc/*.inc``), compiled as six translation units (``-DDP_PART=1..6``) by concurrent hipcc
+    processes and linked into the one library — 26 s of wall time instead of 75 on 8 cores."""
     if not force and not needs_build():
         return LIB_PATH
     from concurrent.futures import ThreadPoolExecutor

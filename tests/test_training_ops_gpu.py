@@ -354,6 +354,12 @@ def test_policy_loss(shape, V, kl, ent, weighted, dtype):
     assert torch.equal(work, d)
 
 
+@pytest.mark.parametrize("rows,V,dtype", [(2, v, "fp32") for v in (1024, 1025, 2048, 2049, 4096, 4097, 8192, 8193, 16384, 16385, 32768, 32769)]
+                         + [(3, v, "bf16") for v in (2047, 4095, 8191, 16383, 32767, 65535)] + [(66, 33003, "fp32")])
+def test_policy_loss_where_the_row_length_changes_the_kernel(rows, V, dtype):
+    test_policy_loss((rows,), V, 0.04, 0.01, True, dtype)
+
+
 def test_policy_loss_on_its_own_draws_and_its_clip():
     """ratio = 1 (the first step after the draw): the gradient of the plain branch; far outside the range: none on the clipped
     side, the plain one on the other."""
