@@ -1,0 +1,86 @@
+"""Calls of ops.label_logprob / preference_loss / policy_loss, optim.AdamW and generate(update="adamw") at the edges of what they take.
+
+test_training_edges_emu.py runs the same tests on CPU tensors through the host emulation of the kernels, test_training_edges_asan.py under
+AddressSanitizer.  Tolerances: those of test_training_ops_gpu.py."""
+import pytest
+import torch
+
+from dorpatch_amd import ops
+from test_training_ops_gpu import DTYPES, INF, LOG_S, U, check_grad, check_logp, onehot, policy64, preference64, rand, softmax64
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+# ---------------------------------------------------------------- logits of every magnitude
+MAGNITUDES = [2.0 ** 20, 2.0 ** 22 - 1, 2.0 ** 22, 2.0 ** 24 + 2, 1e9, 2.0 ** 30, 3e9, 1e10, 1e18, 1e20, 1e30, 2.0 ** 100, 2.0 ** 101, 1e38]
+
+
+def large_rows(V, dtype, few):
+    """(logits, labels): for each magnitude of either sign a row of it alone; of it and its neighbour below; ordinary logits beside a
+    negative fill in the first half, in every other column, everywhere but at three entries; ordinary logits under one that large."""
+    t = DTYPES[dtype]
+    base = rand(V, seed=V, scale=3.0)
+    rows, labels = [], []
+    for k, big in enumerate(MAGNITUDES[::3] if few else MAGNITUDES):
+        y = (37 * k + 1) % V
+        big = torch.tensor(big).to(t).item()
+        for a in (big, -big):
+            alone = torch.full((V,), a)
+            # the next value of the type away from zero or towards it, whichever is below
+            below = torch.tensor(a).to(t).view(torch.int32 if dtype == "fp32" else torch.int16)
+            below = (below + (1 if a < 0 else -1)).view(t).float()
+            pair = alone.clone()
+            pair[1::4] = below
+            pair[y] = a
+            rows += [alone, pair]
+        first, every, most, under = base.clone(), base.clone(), torch.full((V,), -big), base.clone()
+        first[:V // 2] = -big
+        every[::2] = -big
+        most[[0, V // 3, V - 1]] = base[:3]
+        under[V // 2] = big
+        for r in (first, every, most):
+            r[y] = 0.25
+        under[y] = 0.25 if y != V // 2 else big
+        rows += [first, every, most, under]
+        labels += [y] * 8
+    x = torch.stack(rows).to(t)
+    assert torch.isfinite(x).all()
+    return x, torch.tensor(labels)
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("V,few,repeat", [(300, False, 1), (2520, False, 1), (9001, True, 1), (40003, True, 1), (33003, True, 2)])
+def test_logits_of_every_magnitude(V, few, repeat, dtype):
+    """Statistics a wave, a workgroup and slices a row; the policy loss in registers, walked twice (33003: 80 rows), and in slices."""
+    x, y = large_rows(V, dtype, few)
+    x, y = x.repeat(repeat, 1), y.repeat(repeat)
+    R = len(y)
+    xd, yd = x.to(DEV), y.to(DEV)
+    p, want, entropy, _ = softmax64(x, y)
+    logp, ent, stats = ops.label_logprob(xd, yd, want_entropy=True)
+    check_logp(logp, want), check_logp(ent, entropy)
+    g = rand(R, seed=3)
+    check_grad(ops.label_logprob_bwd(xd, yd, stats, g.to(DEV)), g.double()[:, None] * (onehot(y, V) - p), g, p, y, dtype)
+    old = (want.clamp(min=-30) - 0.05).float()           # in the clip range, or (the label far under the others) a ratio of 0
+    adv, ref = rand(R, seed=4), (want.clamp(min=-30) + 0.1).float()
+    weight = torch.where(want < -30, 0.0, 1.0)           # a label that far down has no part in the loss; exp(ref - logp) would be infinite
+    ref = torch.where(want < -30, -INF, ref)
+    loss, d, lp, h = ops.policy_loss(xd, yd, old.to(DEV), adv.to(DEV), 0.2, 0.28, 0.9, ref_logp=ref.to(DEV), kl_coef=0.04, entropy_coef=0.01, weight=weight.to(DEV))
+    wl, wd, wlp, wh, slope, _ = policy64(x, y, old, adv, 0.2, 0.28, 0.9, ref, 0.04, 0.01, weight)
+    check_logp(lp, wlp), check_logp(h, wh)
+    live = want >= -30
+    # as in test_policy_loss: the ratios are off by LOG_S of themselves and four roundings
+    off = (adv.abs().double() * torch.exp(wlp - old.double()) + 0.04 * (1 + torch.exp(ref.double() - wlp))) * (LOG_S + 4 * U)
+    assert ((loss.cpu().double() - wl).abs() <= off + 0.01 * 2 * LOG_S + 4 * U * (wl.abs() + 0.01 * wh))[live].all()
+    check_grad(d.cpu()[live], wd[live], slope[live], p[live], y[live], dtype, g_err=(0.9 * off + 4 * U * slope.abs())[live], entropy=(0.9 * weight * 0.01)[live])
+    assert torch.isfinite(d).all() and (d.cpu()[~live] == 0).all()
+    keep = live.nonzero()[:, 0]
+    keep = keep[:len(keep) // 2 * 2]
+    xs, ys = x[keep], y[keep]
+    cu = torch.arange(len(keep) + 1, dtype=torch.int32)
+    loss, d, seq = ops.preference_loss(xs.to(DEV), ys.to(DEV), cu.to(DEV), None, 0.3, 0.5)
+    wl, wd, ws, slope, _ = preference64(xs, ys, cu.tolist(), None, 0.3, 0.0, False, 0.5)
+    check_logp(seq, ws)
+    assert ((loss.cpu().double() - wl).abs() <= 0.6 * LOG_S + 2 * U * wl.abs()).all()
+    check_grad(d, wd, slope, p[keep], ys, dtype, g_err=0.5 * 0.3 * 0.6 * LOG_S / 4 + 2 * U * slope.abs())
