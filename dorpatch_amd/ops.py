@@ -355,6 +355,12 @@ def _dlogits(logits, d, out):
     return out, _rows(out, "out")[0]
 
 
+def _wrote(out):
+    """After a launch that wrote into the caller's ``out`` (None: into a tensor of its own): autograd has to know."""
+    if out is not None and not out.is_inference():
+        torch.autograd.graph.increment_version(out)
+
+
 def _extent(t):
     return (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size() if t.numel() else 0
 
@@ -391,11 +397,12 @@ def label_logprob_bwd(logits, labels, stats, g, out=None):
     lib = _lib.load()
     d, rows, shape = _logits(logits, labels)
     _per_row(stats, (rows, 2), labels, "stats"), _per_row(g, shape, labels, "g")
-    out, od = _dlogits(logits, d, out)
+    dlogits, od = _dlogits(logits, d, out)
     if rows:
         _lib.check(lib.dp_label_logprob_bwd(ctypes.byref(d), labels.data_ptr(), stats.data_ptr(), g.data_ptr(), ctypes.byref(od),
                                             _stream()), "dp_label_logprob_bwd")
-    return out
+        _wrote(out)
+    return dlogits
 
 
 def preference_loss(logits, labels, cu_seqlens, ref_logp, beta, upstream, label_smoothing=0.0, average=False, want_grad=True,
@@ -433,6 +440,8 @@ def preference_loss(logits, labels, cu_seqlens, ref_logp, beta, upstream, label_
                                       float(upstream), float(label_smoothing), 1 if average else 0, loss.data_ptr(),
                                       seq_logp.data_ptr(), ctypes.byref(od) if want_grad else None, _ptr(work), _stream()),
                "dp_preference_loss")
+    if want_grad:
+        _wrote(out)
     return loss, dlogits, seq_logp
 
 
@@ -467,6 +476,8 @@ def policy_loss(logits, labels, old_logp, advantage, clip_low, clip_high, upstre
                                       advantage.data_ptr(), _ptr(ref_logp), _ptr(weight), loss.data_ptr(), logp.data_ptr(),
                                       _ptr(entropy), ctypes.byref(od) if want_grad else None, _ptr(work), _stream()),
                    "dp_policy_loss")
+        if want_grad:
+            _wrote(out)
     return loss, dlogits, logp, entropy
 
 

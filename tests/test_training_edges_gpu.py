@@ -84,3 +84,36 @@ def test_logits_of_every_magnitude(V, few, repeat, dtype):
     check_logp(seq, ws)
     assert ((loss.cpu().double() - wl).abs() <= 0.6 * LOG_S + 2 * U * wl.abs()).all()
     check_grad(d, wd, slope, p[keep], ys, dtype, g_err=0.5 * 0.3 * 0.6 * LOG_S / 4 + 2 * U * slope.abs())
+
+
+# ---------------------------------------------------------------- gradients written into the caller's tensors
+def loss_calls(y, r, cu):
+    """The losses' calls that write into `out`, by name."""
+    return {"label_logprob_bwd": lambda x, out: ops.label_logprob_bwd(x, y, ops.label_logprob(x, y)[2], r, out=out),
+            "preference_loss": lambda x, out: ops.preference_loss(x, y, cu, None, 0.3, 1.0, out=out)[1],
+            "policy_loss": lambda x, out: ops.policy_loss(x, y, r, r, 0.2, 0.2, 1.0, out=out)[1]}
+
+
+@pytest.mark.parametrize("name", sorted(loss_calls(None, None, None)))
+def test_autograd_notices_a_gradient_written_over_the_logits(name):
+    """What an operation before the logits has kept of them is gone: its backward has to say so, not to use the gradient in its place."""
+    y, r, cu = torch.tensor([1, 2, 3, 4]).to(DEV), torch.full((4,), -2.0).to(DEV), torch.tensor([0, 2, 4], dtype=torch.int32).to(DEV)
+    call = loss_calls(y, r, cu)[name]
+    w = rand(6, 9, seed=1).to(DEV).requires_grad_(True)
+    h = rand(4, 6, seed=2).to(DEV)
+    x = torch.tanh(h @ w)                           # (its backward takes its result)
+    before = x._version
+    want = call(x.detach(), None)
+    assert x._version == before                     # a gradient of its own: nothing of the caller's was written
+    d = call(x.detach(), x.detach())
+    assert torch.equal(d, want) and torch.equal(x.detach(), want) and x._version > before
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        x.backward(d.clone())
+    other = torch.zeros(4, 12).to(DEV)
+    z = (other * w[0, 0]).sum()                     # keeps `other` for the backward of w
+    call(want.clone(), other[:, 1:10])
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.backward()
+    with torch.inference_mode():
+        x = rand(4, 9, seed=3).to(DEV)
+        assert torch.equal(call(x, x), x)
