@@ -117,3 +117,16 @@ def test_autograd_notices_a_gradient_written_over_the_logits(name):
     with torch.inference_mode():
         x = rand(4, 9, seed=3).to(DEV)
         assert torch.equal(call(x, x), x)
+
+
+@pytest.mark.parametrize("cu", [[0, 2147483647, 5], [2147483647, 5, 6], [2147483600, 2147483647, 3], [0, 2147483584, -1], [-2147483648, 2147483647, 2147483647]])
+def test_sequences_that_start_behind_every_row(cu):
+    """Bounds that are no row at all name no rows: what is inside the tensors counts, and a start near 2^31 does not wrap round."""
+    x, y = rand(6, 40, seed=1).to(DEV), torch.ones(6, dtype=torch.int64).to(DEV)
+    bounds = torch.tensor(cu, dtype=torch.int32).to(DEV)
+    want = softmax64(x, y)[1].sum()
+    for grad in (False, True):
+        loss, d, seq = ops.preference_loss(x, y, bounds, None, 0.1, 1.0, want_grad=grad)
+        assert torch.isfinite(loss).all() and (d is None or torch.isfinite(d).all())
+        if cu[0] <= 0 and cu[2] >= 6:               # the first sequence holds all rows
+            assert abs(float(seq[0]) - float(want)) <= 6 * LOG_S + 2 * U * abs(float(want)) and seq[1] == 0
