@@ -284,7 +284,8 @@ class DorPatch(object):
         (EXTENSION, not in the reference: ``"adamw"`` — pattern and mask of every image follow their gradients through
         ``dorpatch_amd.optim.AdamW`` without decay, lr as the schedule has it, clamped to [clip_min, clip_max], moments
         from zero in each stage; ``"sign"``, the default: the reference's signed update, ``attack.py:333-342``),
-        ``adamw`` (a dict of that optimiser's ``betas``, ``eps``, ``state_bits``, ``seed``).
+        ``adamw`` (a dict of that optimiser's ``betas``, ``eps``, ``state_bits``, ``seed``; they are in the names of its stage-0
+        cache files, whose plain names are the signed update's).
         """
         run = HotLoop(self, model, x, patch_budget, n_classes, save_dir, batch_id, y, targeted, lr,
                       confidence, clip_min, clip_max, max_iterations, basic_unit, selection, dropout,
@@ -544,9 +545,10 @@ class HotLoop(object):
         self.update = extras.get("update", "sign")
         if self.update not in ("sign", "adamw"):
             raise ValueError("update must be 'sign' or 'adamw' (got %r)" % (self.update,))
-        self._adamw_args = dict(extras.get("adamw", {}))
-        if not set(self._adamw_args) <= {"betas", "eps", "state_bits", "seed"}:
-            raise ValueError("adamw takes betas, eps, state_bits, seed (got %s)" % sorted(self._adamw_args))
+        self._adamw_args = dict(betas=(0.9, 0.999), eps=1e-8, state_bits=32, seed=0)
+        if not set(extras.get("adamw", {})) <= set(self._adamw_args):
+            raise ValueError("adamw takes betas, eps, state_bits, seed (got %s)" % sorted(extras["adamw"]))
+        self._adamw_args.update(extras.get("adamw", {}))
         self._adamw = None
 
         self.net, self.norm = _unwrap_model(model)
@@ -717,6 +719,15 @@ class HotLoop(object):
         parts = self.save_dir.split('/')[:-1]                          # attack.py:103
         return os.path.join(*parts) if parts else "."
 
+    def _stage0_files(self, dir_0):
+        """(mask, pattern) of the stage-0 cache.  The reference's names are the signed update's; what AdamW made carries its arguments,
+        so that no run takes up another update's first stage."""
+        tag = ""
+        if self.update == "adamw":
+            a = self._adamw_args
+            tag = "adamw-%r-%r-%r-%d-%d_" % (float(a["betas"][0]), float(a["betas"][1]), float(a["eps"]), a["state_bits"], int(a["seed"]))
+        return tuple(os.path.join(dir_0, "adv_%s_%s%d.pt" % (name, tag, self.batch_id)) for name in ("mask", "pattern"))
+
     def _flags(self, attr):
         return np.array([getattr(s, attr) for s in self.img], dtype=bool)
 
@@ -758,12 +769,11 @@ class HotLoop(object):
             for s in self.img:
                 s.reset_stage()
                 s.steps_in_stage = 0        # per stage, not per reset: the untargeted -> targeted switch resets mid-stage
-            mpath = os.path.join(dir_0, "adv_mask_%d.pt" % self.batch_id)
+            mpath, ppath = self._stage0_files(dir_0)
             # every rank follows rank 0's view of the cache (skipping stage 0 on one rank only would deadlock)
             if stage == 0 and dp_dist.broadcast_object(os.path.exists(mpath), o.pg):   # attack.py:134-141
                 self.best_mask = torch.load(mpath, map_location=self.dev).float().contiguous()
-                self.best_pattern = torch.load(os.path.join(dir_0, "adv_pattern_%d.pt" % self.batch_id),
-                                               map_location=self.dev).float().contiguous()
+                self.best_pattern = torch.load(ppath, map_location=self.dev).float().contiguous()
                 continue
             t0 = self._clock()
             if stage == 1:
@@ -812,8 +822,8 @@ class HotLoop(object):
         if stage == 0:
             if self.rank == 0:                                         # :351-356 stage-0 cache (pattern first:
                 os.makedirs(dir_0, exist_ok=True)                      # the mask file's presence means "complete")
-                for name, t in (("adv_pattern_%d.pt", self.best_pattern), ("adv_mask_%d.pt", self.best_mask)):
-                    path = os.path.join(dir_0, name % self.batch_id)
+                mpath, ppath = self._stage0_files(dir_0)
+                for path, t in ((ppath, self.best_pattern), (mpath, self.best_mask)):
                     torch.save(t, path + ".tmp")
                     os.replace(path + ".tmp", path)
             if not all(self._flags("flag_targeted")) and last_i >= 0:  # :357-359 (set_target(preds_adv, y))

@@ -3,6 +3,7 @@ import importlib.util
 import os
 
 import pytest
+import torch
 
 from tests_hipemu import patch as emu_patch
 
@@ -18,7 +19,8 @@ _mod.DEV = "cpu"
 
 
 @pytest.fixture(autouse=True)
-def _emulated():
+def _emulated(monkeypatch):
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda *a, **k: None)
     with emu_patch.emulated_ops():
         yield
 

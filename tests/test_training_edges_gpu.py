@@ -2,10 +2,14 @@
 
 test_training_edges_emu.py runs the same tests on CPU tensors through the host emulation of the kernels, test_training_edges_asan.py under
 AddressSanitizer.  Tolerances: those of test_training_ops_gpu.py."""
+import numpy as np
 import pytest
 import torch
 
 from dorpatch_amd import ops
+from dorpatch_amd.attack import DorPatch
+from dorpatch_amd.utils import NormModel, get_normalize
+from oracle import toy_models
 from test_training_ops_gpu import DTYPES, INF, LOG_S, U, check_grad, check_logp, onehot, policy64, preference64, rand, softmax64
 
 pytestmark = pytest.mark.gpu
@@ -130,3 +134,42 @@ def test_sequences_that_start_behind_every_row(cu):
         assert torch.isfinite(loss).all() and (d is None or torch.isfinite(d).all())
         if cu[0] <= 0 and cu[2] >= 6:               # the first sequence holds all rows
             assert abs(float(seq[0]) - float(want)) <= 6 * LOG_S + 2 * U * abs(float(want)) and seq[1] == 0
+
+
+# ---------------------------------------------------------------- the attack's AdamW
+def attack(stages=None, n_it=2, B=1, hook=None, **extra):
+    """A short run on one directory's path: (mask, pattern) on the CPU; `stages`: the stage of every step."""
+    H = 56
+    model = NormModel(toy_models.make_toy(gain=2.0), get_normalize("imagenet", "resnetv2")).to(DEV)
+    g = torch.Generator().manual_seed(5)
+    x = torch.rand(B, 3, H, H, generator=g).to(DEV)
+
+    def seen(d):
+        if stages is not None:
+            stages.append(int(d["stage"]))
+        if hook is not None:
+            hook(d)
+    extra.setdefault("init_mask", torch.rand(B, 1, H, H, generator=g))
+    out = DorPatch(verbose=False).generate(model, x, 0.12, 10, "res/cfg/sub", 0, y=torch.arange(1, B + 1).to(DEV), targeted=True, lr=0.01, sampling_size=4,
+                                           max_iterations=n_it, init_pattern=torch.rand(B, 3, H, H, generator=g),
+                                           rngs=[np.random.RandomState(b) for b in range(B)], step_hook=seen, **extra)
+    return [t.cpu() for t in out]
+
+
+@pytest.mark.parametrize("first,second", [(dict(), dict(update="adamw")), (dict(update="adamw"), dict()),
+                                          (dict(update="adamw", adamw=dict(state_bits=8, seed=3)), dict(update="adamw", adamw=dict(state_bits=8, seed=4)))])
+def test_attack_stage_0_of_another_update_is_not_taken_for_ones_own(tmp_path, monkeypatch, first, second):
+    """Two runs in one directory: each has its own first stage, and gives what it gives alone; a run again takes its own up."""
+    for name in ("alone", "both"):
+        (tmp_path / name).mkdir()
+    monkeypatch.chdir(tmp_path / "alone")
+    alone = attack(**second)
+    monkeypatch.chdir(tmp_path / "both")
+    attack(**first)
+    stages = []
+    got = attack(stages, **second)
+    assert stages == [0, 0, 1, 1] and all(torch.equal(a, b) for a, b in zip(got, alone))
+    for options in (first, second):
+        stages = []
+        attack(stages, **options)
+        assert stages == [1, 1]
