@@ -283,7 +283,7 @@ class DorPatch(object):
         patch under its own random affine placement; ``None`` = the reference's identity placement), ``update``
         (EXTENSION, not in the reference: ``"adamw"`` — pattern and mask of every image follow their gradients through
         ``dorpatch_amd.optim.AdamW`` without decay, lr as the schedule has it, clamped to [clip_min, clip_max], moments
-        from zero in each stage; ``"sign"``, the default: the reference's signed update, ``attack.py:333-342``),
+        from zero in each stage, a gradient that is not finite taken for 0; ``"sign"``, the default: the reference's signed update, ``attack.py:333-342``),
         ``adamw`` (a dict of that optimiser's ``betas``, ``eps``, ``state_bits``, ``seed``; they are in the names of its stage-0
         cache files, whose plain names are the signed update's).
         """
@@ -1014,8 +1014,10 @@ class HotLoop(object):
 
     def _adamw_update(self, g_pattern, g_mask, lr):
         """AdamW on every image's pattern (stage 0: and mask), each with its image's lr (0: finished).  The gradient of a mask cell
-        that is all 0 is NaN, which the signed update freezes at 0 (sign(NaN) = 0): here it counts as 0 and the cell stays."""
-        learned = [(self.adv_pattern, g_pattern)] + ([(self.adv_mask, torch.nan_to_num(g_mask, nan=0.0))] if self.stage == 0 else [])
+        that is all 0 is NaN, which the signed update freezes at 0 (sign(NaN) = 0): here it counts as 0 and the cell stays.  So does
+        an infinite one (a cell whose squares underflow): in the moments it would stay for good."""
+        learned = [(self.adv_pattern, g_pattern)] + ([(self.adv_mask, g_mask)] if self.stage == 0 else [])
+        learned = [(p, torch.nan_to_num(g, nan=0.0, posinf=0.0, neginf=0.0)) for p, g in learned]
         if self._adamw is None or self._adamw[0] != self.stage:
             from . import optim
             self._adamw = (self.stage, optim.AdamW([p[b] for p, _ in learned for b in range(self.B)], weight_decay=0.0,

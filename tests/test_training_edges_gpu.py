@@ -173,3 +173,30 @@ def test_attack_stage_0_of_another_update_is_not_taken_for_ones_own(tmp_path, mo
         stages = []
         attack(stages, **options)
         assert stages == [1, 1]
+
+
+def test_attack_adamw_takes_a_gradient_that_is_not_finite_for_none(tmp_path, monkeypatch):
+    """One step's gradient holds infinities and a NaN: there it counts as 0 in pattern and mask, and both go on as by the formula."""
+    monkeypatch.chdir(tmp_path)
+    seen, bad = [], [(0, 20, 30, INF), (1, 33, 9, -INF), (2, 41, 40, float("nan"))]
+
+    def plant(d):
+        seen.append({k: (d[k].detach().cpu().clone() if torch.is_tensor(d[k]) else np.array(d[k])) for k in ("stage", "grad_pattern", "grad_mask", "mask", "pattern", "lr")})
+        if d["i"] == 1:
+            for c, h, w, value in bad:
+                d["g_adv"][0, c, h, w] = value
+                seen[-1]["grad_pattern"][0, c, h, w] = seen[-1]["grad_mask"][0, 0, h, w] = 0.0
+    attack(n_it=4, hook=plant, update="adamw", adamw=dict(betas=(0.8, 0.95)))
+    for name, learned_in in (("pattern", (0, 1)), ("mask", (0,))):
+        for stage in learned_in:
+            steps = [d for d in seen if d["stage"] == stage]
+            m = v = torch.zeros_like(steps[0][name]).double()
+            for t, (d, after) in enumerate(zip(steps, steps[1:]), 1):
+                g = d["grad_" + name].double().nan_to_num(nan=0.0)
+                m, v = 0.8 * m + 0.2 * g, 0.95 * v + 0.05 * g * g
+                lr = torch.from_numpy(d["lr"]).double().view(-1, 1, 1, 1)
+                change = lr * (m / (1 - 0.8 ** t)) / ((v / (1 - 0.95 ** t)).sqrt() + 1e-8)
+                want = (d[name].double() - change).clamp(0, 1)
+                # as in test_pattern_and_mask_follow_adamw
+                assert ((after[name].double() - want).abs() <= 2 * U * (want.abs() + d[name].abs()) + (3 * t + 8) * U * (change.abs() + lr)).all(), (name, stage, t)
+    assert len(seen) == 8 and all(torch.isfinite(d[k]).all() for d in seen for k in ("pattern", "mask"))
