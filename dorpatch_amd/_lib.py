@@ -22,6 +22,7 @@ DP_DEBUG_CONV3X3_VARIANT = 6
 DP_S2BWD_PAIRS, DP_S2BWD_CLASSES = 0, 1      # dp_conv3x3s2_bwd forms
 DP_F32, DP_BF16, DP_F16 = 0, 1, 2            # element types of logits, parameters, gradients
 DP_LOGPROB, DP_PREFERENCE, DP_POLICY = 0, 1, 2   # dp_logits_workspace's operators
+DP_MAX_ROWS, DP_MAX_VOCAB, DP_MAX_PAIRS = 1 << 23, 1 << 30, (1 << 24) - 1    # what the losses on logits take
 DP_ADAMW_BLOCK = 128                         # elements that share a scale of AdamW's 8-bit states
 
 c_float_p = ctypes.c_void_p  # device pointers travel as integers

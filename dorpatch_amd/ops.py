@@ -305,6 +305,8 @@ def _rows(x, name="logits"):
         rows, inner, outer, row = shape[0] * shape[1], shape[1], stride[0], stride[1]
     else:
         rows, inner, outer, row = 1, 1, 0, 0
+    if rows > _lib.DP_MAX_ROWS or V > _lib.DP_MAX_VOCAB:     # (a C int would silently be another size)
+        raise ValueError("`%s` may have up to 2^23 rows and 2^30 categories, got %d and %d" % (name, rows, V))
     return _lib.DpLogits(x.data_ptr(), kind, rows, V, inner or 1, outer, row), rows
 
 
@@ -405,6 +407,15 @@ def label_logprob_bwd(logits, labels, stats, g, out=None):
     return dlogits
 
 
+def _pairs(cu_seqlens):
+    if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1 or cu_seqlens.shape[0] % 2 != 1:
+        raise ValueError("`cu_seqlens` must be (2 * pairs + 1,), got %s" % (tuple(cu_seqlens.shape),))
+    P = cu_seqlens.shape[0] // 2
+    if P > _lib.DP_MAX_PAIRS:
+        raise ValueError("`cu_seqlens` may have up to 2^24 - 1 pairs, got %d" % P)
+    return P
+
+
 def preference_loss(logits, labels, cu_seqlens, ref_logp, beta, upstream, label_smoothing=0.0, average=False, want_grad=True,
                     out=None):
     """Preference loss over pairs of sequences (paired log ratios) and its gradient: (loss (P,), dlogits or None, seq_logp (2P,)).
@@ -420,9 +431,7 @@ def preference_loss(logits, labels, cu_seqlens, ref_logp, beta, upstream, label_
     if logits.dim() != 2:
         raise ValueError("`logits` must be (R, V): the sequences lie one after the other")
     _chk(cu_seqlens, torch.int32, "cu_seqlens"), _beside(cu_seqlens, labels, "cu_seqlens")
-    if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1 or cu_seqlens.shape[0] % 2 != 1:
-        raise ValueError("`cu_seqlens` must be (2 * pairs + 1,), got %s" % (tuple(cu_seqlens.shape),))
-    P = cu_seqlens.shape[0] // 2
+    P = _pairs(cu_seqlens)
     _per_row(ref_logp, (2 * P,), labels, "ref_logp")
     if not 0.0 <= label_smoothing <= 1.0:
         raise ValueError("`label_smoothing` must be in [0, 1], got %r" % (label_smoothing,))

@@ -200,3 +200,22 @@ def test_attack_adamw_takes_a_gradient_that_is_not_finite_for_none(tmp_path, mon
                 # as in test_pattern_and_mask_follow_adamw
                 assert ((after[name].double() - want).abs() <= 2 * U * (want.abs() + d[name].abs()) + (3 * t + 8) * U * (change.abs() + lr)).all(), (name, stage, t)
     assert len(seen) == 8 and all(torch.isfinite(d[k]).all() for d in seen for k in ("pattern", "mask"))
+
+
+# ---------------------------------------------------------------- sizes beyond the kernels' own numbers
+def test_losses_refuse_sizes_that_do_not_fit_their_32_bits():
+    """A row of 2^32 + 8 categories is none of 8, nor 2^32 + 1 pairs one: the sizes are looked at before they become C integers.  (The
+    tensors are broadcast or lie on the meta device: no memory is behind them.)"""
+    def refused(match, call, *a, **k):
+        with pytest.raises(ValueError, match=match):
+            call(*a, **k)
+    y = torch.tensor(3).to(DEV)
+    for V in (2 ** 30 + 1, 2 ** 31, 2 ** 32 + 8):
+        refused("categories", ops._rows, torch.empty(V, dtype=torch.bfloat16, device="meta"))
+    for rows in (2 ** 23 + 1, 2 ** 31, 2 ** 32 + 5):
+        refused("rows", ops._rows, torch.zeros(1, 1).to(DEV).expand(rows, 1))
+        refused("rows", ops._rows, torch.zeros(1, 1, 1).to(DEV).expand(2, rows, 1))
+    x = torch.zeros(4, 8).to(DEV)
+    for pairs in (2 ** 24, 2 ** 31, 2 ** 32 + 1):
+        refused("pairs", ops._pairs, torch.empty(2 * pairs + 1, dtype=torch.int32, device="meta"))
+    assert ops._rows(x)[1] == 4 and ops._pairs(torch.zeros(5, dtype=torch.int32)) == 2
