@@ -442,7 +442,8 @@ int dp_label_logprob_bwd(const dp_logits_t *x, const int64_t *labels, const floa
                          dp_stream_t stream);
 
 /* Preference loss of pairs of sequences.  Sequence k is the rows [cu_seqlens[k], cu_seqlens[k + 1]) (int32, 2 * pairs + 1
- * ascending values; empty ones and rows outside are fine), 2 i the preferred and 2 i + 1 the other of pair i.
+ * ascending values; empty ones and rows outside are fine; 2 i the preferred and 2 i + 1 the other of pair i;
+ * values that are no rows are clamped to them).  pairs < 2^24.
  *   L_k = sum over its rows that count of log softmax(x)[label]  (average: their mean; 0 for none)       -> seq_logp (2 pairs)
  *   h_i = beta * ((L_2i - ref_logp[2i]) - (L_2i+1 - ref_logp[2i+1]))          (ref_logp NULL: 0)
  *   loss[i] = -(1 - label_smoothing) log sigmoid(h_i) - label_smoothing log sigmoid(-h_i)

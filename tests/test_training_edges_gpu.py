@@ -219,3 +219,15 @@ def test_losses_refuse_sizes_that_do_not_fit_their_32_bits():
     for pairs in (2 ** 24, 2 ** 31, 2 ** 32 + 1):
         refused("pairs", ops._pairs, torch.empty(2 * pairs + 1, dtype=torch.int32, device="meta"))
     assert ops._rows(x)[1] == 4 and ops._pairs(torch.zeros(5, dtype=torch.int32)) == 2
+
+
+def test_c_entry_refuses_more_pairs_than_a_launch_takes():
+    """2^24 workgroups of 256 are 2^32 threads, one more than a launch has."""
+    import ctypes
+    from dorpatch_amd import _lib
+    lib, P = _lib.load(), ctypes.c_void_p
+    x, y, o = torch.zeros(4, 8).to(DEV), torch.zeros(4, dtype=torch.int64).to(DEV), torch.zeros(64).to(DEV)
+    d = _lib.DpLogits(data=x.data_ptr(), dtype=0, rows=4, vocab=8, inner=4, outer_stride=0, row_stride=8)
+    for pairs in (2 ** 24, 2 ** 30, 2 ** 31 - 1, 0, -1):        # (nothing is read of what the pointers name)
+        assert lib.dp_preference_loss(ctypes.byref(d), P(y.data_ptr()), P(y.data_ptr()), pairs, None, 0.1, 1.0, 0.0, 0, P(o.data_ptr()), P(o.data_ptr()), None,
+                                      P(o.data_ptr()), ops._stream()) == 1, pairs
