@@ -141,6 +141,7 @@ class AdamW(object):
 
     def step(self, grads=None, lr=None):
         """One step from ``grads`` (a list; None: every parameter's ``.grad``; an entry None: that tensor stays), in place.
+        A gradient may not lie on a parameter that the step writes, but for its own as a whole.
         ``lr``: a number or one for each tensor, for this and the next steps.  Returns the global gradient norm before clipping
         (a 0-dim float32 tensor) where ``max_norm`` is set, else None."""
         lib = _lib.load()

@@ -482,7 +482,8 @@ int dp_policy_loss(const dp_policy_cfg_t *cfg, const dp_logits_t *x, const int64
  * t: step if counter is NULL; else the int64 on the device is advanced by one first and taken (captured graphs: it advances on
  *   every replay).  max_norm > 0 needs it: clip = min(1, max_norm / (norm + 1e-6)) with norm = sqrt(sum of all g^2), summed in
  *   fp64 in a fixed order -> *norm.  Where norm is not finite nothing is changed, t neither.
- * workspace: dp_adamw_workspace() bytes, 16-byte aligned.  Refused (hipErrorInvalidValue): params that overlap, states that do. */
+ * workspace: dp_adamw_workspace() bytes, 16-byte aligned.  Refused (hipErrorInvalidValue): params that overlap, states that do, a
+ * grad that overlaps a param (but one that is its own param, of the same type). */
 #define DP_ADAMW_BLOCK 128
 typedef struct {
   void *param;

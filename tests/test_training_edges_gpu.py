@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 import torch
 
-from dorpatch_amd import ops
+from dorpatch_amd import ops, optim
 from dorpatch_amd.attack import DorPatch
 from dorpatch_amd.utils import NormModel, get_normalize
 from oracle import toy_models
@@ -231,3 +231,28 @@ def test_c_entry_refuses_more_pairs_than_a_launch_takes():
     for pairs in (2 ** 24, 2 ** 30, 2 ** 31 - 1, 0, -1):        # (nothing is read of what the pointers name)
         assert lib.dp_preference_loss(ctypes.byref(d), P(y.data_ptr()), P(y.data_ptr()), pairs, None, 0.1, 1.0, 0.0, 0, P(o.data_ptr()), P(o.data_ptr()), None,
                                       P(o.data_ptr()), ops._stream()) == 1, pairs
+
+
+# ---------------------------------------------------------------- AdamW
+def test_adamw_refuses_gradients_that_lie_on_parameters():
+    """A step writes its parameters while others of its workgroups still read gradients: a gradient on another parameter, or askew on
+    its own, would be read before or after, as it happens.  A parameter that is its own gradient is read where it is written."""
+    def parameters():
+        return [torch.full((5000,), 1.0).to(DEV), torch.full((5000,), 2.0).to(DEV), torch.full((300,), 3.0).to(DEV)]
+    one = torch.ones(5000).to(DEV)
+    for max_norm in (None, 1.0):
+        a, b, c = parameters()
+        opt = optim.AdamW([a, b, c], weight_decay=0.0, max_norm=max_norm)
+        for grads in ([b, a, c], [one, a, None], [one, one, b[4000:4300]], [one, one, a[:300]]):
+            with pytest.raises(RuntimeError, match="dp_adamw_step"):
+                opt.step(grads)
+        flat = torch.ones(5001).to(DEV)
+        askew = optim.AdamW([flat[1:]], max_norm=max_norm)
+        with pytest.raises(RuntimeError, match="dp_adamw_step"):
+            askew.step([flat[:-1]])
+        assert opt.steps == askew.steps == 0 and (flat == 1).all()
+        assert all(torch.equal(p, q) for p, q in zip((a, b, c), parameters()))
+        opt.step([a, None, b[:300]])                # its own; a parameter that this step does not write
+        assert (b == 2).all() and opt.steps == 1
+        for p, before in ((a, 1.0), (c, 3.0)):      # step 1 moves an element by lr against its gradient's sign
+            assert ((p - (before - 1e-3)).abs() <= 4 * U * before).all()
