@@ -549,6 +549,8 @@ class HotLoop(object):
         if not set(extras.get("adamw", {})) <= set(self._adamw_args):
             raise ValueError("adamw takes betas, eps, state_bits, seed (got %s)" % sorted(extras["adamw"]))
         self._adamw_args.update(extras.get("adamw", {}))
+        if not self._adamw_args["eps"] >= 2.0 ** -126:       # (a normal float32: a cell that is all 0 would have a step of 0 / 0)
+            raise ValueError("adamw needs an eps > 0 (got %r)" % (self._adamw_args["eps"],))
         self._adamw = None
 
         self.net, self.norm = _unwrap_model(model)

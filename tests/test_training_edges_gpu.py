@@ -256,3 +256,11 @@ def test_adamw_refuses_gradients_that_lie_on_parameters():
         assert (b == 2).all() and opt.steps == 1
         for p, before in ((a, 1.0), (c, 3.0)):      # step 1 moves an element by lr against its gradient's sign
             assert ((p - (before - 1e-3)).abs() <= 4 * U * before).all()
+
+
+def test_attack_adamw_needs_an_eps(tmp_path, monkeypatch):
+    """A cell that is all 0 has no gradient: without eps its step would be 0 / 0."""
+    monkeypatch.chdir(tmp_path)
+    for eps in (0.0, 1e-60, -1e-8, float("nan")):       # (1e-60: 0 in the kernel's 32 bits)
+        with pytest.raises(ValueError, match="eps"):
+            attack(update="adamw", adamw=dict(eps=eps))
