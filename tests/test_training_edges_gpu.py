@@ -264,3 +264,26 @@ def test_attack_adamw_needs_an_eps(tmp_path, monkeypatch):
     for eps in (0.0, 1e-60, -1e-8, float("nan")):       # (1e-60: 0 in the kernel's 32 bits)
         with pytest.raises(ValueError, match="eps"):
             attack(update="adamw", adamw=dict(eps=eps))
+
+
+@pytest.mark.parametrize("V", [300, 2520, 9001, 40003])
+def test_logits_on_both_sides_of_the_far_border(V):
+    """References of 2^22 and more take differences, smaller ones do not: rows whose lanes hold the one and the other are joined."""
+    spread = rand(6, V, seed=V, scale=4.0)
+    x = torch.stack([s * 2.0 ** 22 + spread[k] for k, s in enumerate((1.0, -1.0, 1.0, -1.0, 1.0, -1.0))])
+    x[2:4, ::2] = spread[2:4, ::2]                  # ordinary ones, far below or above
+    x[4, V // 2:] += 16.0                           # ascending and descending borders
+    x[5, :V // 2] -= 16.0
+    y = x.argmax(1)
+    y[1] = 0
+    p, want, entropy, _ = softmax64(x, y)
+    xd, yd = x.to(DEV), y.to(DEV)
+    logp, ent, stats = ops.label_logprob(xd, yd, want_entropy=True)
+    check_logp(logp, want), check_logp(ent, entropy)
+    one = torch.ones(6)
+    check_grad(ops.label_logprob_bwd(xd, yd, stats, one.to(DEV)), onehot(y, V) - p, one, p, y, "fp32")
+    old, adv = want.float(), torch.ones(6)
+    loss, d, lp, h = ops.policy_loss(xd, yd, old.to(DEV), adv.to(DEV), 0.2, 0.2, 1.0, entropy_coef=0.1)
+    wl, wd, wlp, wh, slope, _ = policy64(x, y, old, adv, 0.2, 0.2, 1.0, None, 0.0, 0.1, None)
+    check_logp(lp, wlp), check_logp(h, wh)
+    check_grad(d, wd, slope, p, y, "fp32", g_err=LOG_S + 4 * U, entropy=0.1)
