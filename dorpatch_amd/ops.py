@@ -438,12 +438,15 @@ def preference_loss(logits, labels, cu_seqlens, ref_logp, beta, upstream, label_
     loss = torch.empty((P,), dtype=torch.float32, device=logits.device)
     seq_logp = loss.new_empty((2 * P,))
     dlogits, od = _dlogits(logits, d, out) if want_grad else (None, None)
-    if rows == 0 or P == 0:          # nothing that a kernel would read: sums of nothing
-        seq_logp.zero_()
-        if P:
-            h = float(beta) * (0.0 if ref_logp is None else ref_logp[1::2] - ref_logp[0::2]) + torch.zeros_like(loss)
-            loss.copy_(torch.nn.functional.softplus(-h) + float(label_smoothing) * h)
-        return loss, (dlogits.zero_() if want_grad else None), seq_logp
+    if rows == 0 or P == 0:          # nothing that a kernel would read: sums of nothing, and as from a kernel no part of a graph
+        with torch.no_grad():
+            seq_logp.zero_()
+            if P:
+                h = float(beta) * (0.0 if ref_logp is None else ref_logp[1::2] - ref_logp[0::2]) + torch.zeros_like(loss)
+                loss.copy_(torch.nn.functional.softplus(-h) + float(label_smoothing) * h)
+            if want_grad:
+                dlogits.zero_()
+        return loss, dlogits, seq_logp
     work = _logits_workspace(_lib.DP_PREFERENCE, d, logits.device)
     _lib.check(lib.dp_preference_loss(ctypes.byref(d), labels.data_ptr(), cu_seqlens.data_ptr(), P, _ptr(ref_logp), float(beta),
                                       float(upstream), float(label_smoothing), 1 if average else 0, loss.data_ptr(),

@@ -287,3 +287,19 @@ def test_logits_on_both_sides_of_the_far_border(V):
     wl, wd, wlp, wh, slope, _ = policy64(x, y, old, adv, 0.2, 0.2, 1.0, None, 0.0, 0.1, None)
     check_logp(lp, wlp), check_logp(h, wh)
     check_grad(d, wd, slope, p, y, "fp32", g_err=LOG_S + 4 * U, entropy=0.1)
+
+
+def test_preference_loss_of_nothing_writes_zeroes_into_a_leaf():
+    """No pairs: the gradient is zeroes, written over logits that require one as any other is, and no operation of their graph."""
+    y, cu = torch.tensor([1, 2]).to(DEV), torch.zeros(1, dtype=torch.int32).to(DEV)
+    leaf = rand(2, 9, seed=1).to(DEV).requires_grad_(True)
+    before = leaf._version
+    loss, d, seq = ops.preference_loss(leaf, y, cu, None, 0.3, 1.0, out=leaf)
+    assert d is leaf and (d == 0).all() and loss.numel() == seq.numel() == 0 and leaf.is_leaf and leaf._version > before
+    inner = torch.tanh(rand(2, 9, seed=2).to(DEV).requires_grad_(True))
+    node = inner.grad_fn
+    ops.preference_loss(inner, y, cu, None, 0.3, 1.0, out=inner)
+    assert inner.grad_fn is node and (inner == 0).all()
+    none, ref = torch.zeros(0, 9).to(DEV), torch.tensor([0.5, -1.0]).to(DEV).requires_grad_(True)
+    loss, d, seq = ops.preference_loss(none, y[:0], torch.zeros(3, dtype=torch.int32).to(DEV), ref, 0.3, 1.0)
+    assert not loss.requires_grad and abs(float(loss) - float(torch.nn.functional.softplus(torch.tensor(0.45)))) <= 4 * U
