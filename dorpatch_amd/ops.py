@@ -269,6 +269,7 @@ def cw_loss(logits, y, targeted, S, confidence, upstream, loss_out=None, want_gr
 
 
 # ---------------------------------------------------------------- losses on rows of logits (a training step; not in the reference)
+# As cw_loss they return values and gradients that are no part of an autograd graph: `logits.backward(dlogits)` goes on from there.
 ELEMENT_TYPES = {torch.float32: _lib.DP_F32, torch.bfloat16: _lib.DP_BF16, torch.float16: _lib.DP_F16}
 
 
@@ -379,7 +380,7 @@ def label_logprob(logits, labels, want_entropy=False):
     (``x[:, :-1]`` of a (B, T, V) tensor is taken as it lies); ``labels`` int64 of the rows' shape, a negative one marks a row
     that counts for nothing: it is not read, its outputs are 0 and so is its gradient.  A row that allows nothing (all -inf)
     counts the same; a label beyond the vocabulary gives NaN.  ``logp`` and ``entropy``: float32 of the rows' shape; ``stats``
-    (R, 2): what ``label_logprob_bwd`` needs."""
+    (R, 2): what ``label_logprob_bwd`` needs for the gradient of ``logp`` (``entropy`` has none here; ``policy_loss`` takes its bonus)."""
     lib = _lib.load()
     d, rows, shape = _logits(logits, labels)
     stats = torch.empty((rows, 2), dtype=torch.float32, device=logits.device)
