@@ -414,7 +414,8 @@ int dp_subsample2_add(const float *dy, int64_t NC, int H, int W, float *g, dp_st
  * rows * ceil(bytes of a row / 16384) < 2^24.
  * labels (rows) int64.  A label < 0 marks a row that counts for nothing (a prompt, padding): its logits are not read, its
  * outputs and its gradient are 0 whatever is in it.  So does a row whose logits are all -inf.  A label >= vocab gives NaN in
- * the row's outputs and gradient, and no access.  Single logits may be -inf (not allowed: probability 0).
+ * the row's outputs and gradient, and no access.  Single logits may be -inf (not allowed: probability 0)
+ * or finite and of any magnitude (the type's lowest value as a fill, for one).
  * Gradients go to a tensor `d` of the same type and size, with strides of its own; it may be the logits themselves.
  * Sums are fp32, scalars of a row fp64; no atomics: the same inputs give the same bits.
  * workspace: dp_logits_workspace(op, rows, vocab, dtype) bytes, 16-byte aligned (NULL where that is 0). */
