@@ -417,7 +417,7 @@ int dp_subsample2_add(const float *dy, int64_t NC, int H, int W, float *g, dp_st
  * the row's outputs and gradient, and no access.  Single logits may be -inf (not allowed: probability 0)
  * or finite and of any magnitude (the type's lowest value as a fill, for one).
  * Gradients go to a tensor `d` of the same type and size, with strides of its own; it may be the logits themselves.
- * Sums are fp32, scalars of a row fp64; no atomics: the same inputs give the same bits.
+ * Sums are fp32, logarithms of sums and sums over sequences fp64; no atomics: the same inputs give the same bits.
  * workspace: dp_logits_workspace(op, rows, vocab, dtype) bytes, 16-byte aligned (NULL where that is 0). */
 #define DP_F32 0
 #define DP_BF16 1
